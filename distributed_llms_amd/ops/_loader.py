@@ -9,6 +9,7 @@ raises instead of silently falling back to eager PyTorch.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -55,6 +56,20 @@ def lib() -> ctypes.CDLL:
 
 def stream_ptr() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream(device: torch.device) -> int:
+    """Handle of the current stream of a tensor's device."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which a tensor's device is the current one (kernels launch on the current device); costs nothing where
+    it already is."""
+    return _HERE if torch._C._cuda_getDevice() == t.device.index else torch.cuda.device(t.device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
@@ -120,5 +135,10 @@ def _declare(l: ctypes.CDLL) -> None:
     sig("dlamd_dar_register", [vp, vp, ll, vp])
     sig("dlamd_dar_register_peer", [vp, i, i, vp])
     sig("dlamd_dar_allreduce_region", [vp, i, ll, i, f, i, vp])
+    sig("dlamd_paged_append", [vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, vp, vp, vp, vp]
+        + [i] * 11 + [vp])
+    sig("dlamd_paged_attention", [vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, vp, vp, vp] + [i] * 9 + [f, i, vp])
+    sig("dlamd_verify_draft", [vp, ll, vp, ll, ll, vp, ll, ll, vp, ll, vp, vp, vp, i, i, i, i, i, vp])
+    sig("dlamd_int4_linear", [vp, ll, vp, vp, vp, vp, vp, ll, vp, i, i, i, i, i, i, i, vp])
     sig("dlamd_embed_rows", [vp, vp, vp, vp, vp, ll, i, i, i, i, f, vp])
     sig("dlamd_decode_bookkeep", [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp])

@@ -1,0 +1,141 @@
+"""Linear layers with 4-bit weights and group scales, for the few rows of a decode step.  GPU: csrc/kernels/int4_linear.hip;
+CPU tensors: plain PyTorch fp32 on the dequantized weights (also the oracle).
+
+``quantize_int4`` (from a float weight) or ``pack_int4`` (from codes, scales and zeros made elsewhere) lays a layer's weights
+out once; ``linear_int4`` is then called like ``ops.conv.linear_bf16``.  Weight (n, k) is (code - zero) * scale with codes
+0 .. 15 and one scale (and zero, 8 if none are given) per row and group of G = 32, 64 or 128 input features."""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _loader
+from .conv import _act_ref
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_ACTS = {"none": 0, "relu": 1, "gelu": 3}
+GROUPS = (32, 64, 128)
+
+
+@dataclass
+class Int4Weight:
+    """A layer's weights in the kernels' order.  words: int32 [N / 16, K / 128, 64, 4] (sizes rounded up; lane 16 g + r,
+    word i holds row r of its 16 and the features 32 i + 8 g .. + 8 of its 128, code 2 p in bits 4 p, code 2 p + 1 in bits
+    16 + 4 p); scale: [K / G, N rounded up to 16] bf16 or fp16; zero: uint8 alike, or None (8)."""
+
+    words: torch.Tensor
+    scale: torch.Tensor
+    zero: Optional[torch.Tensor]
+    n: int
+    k: int
+    group: int
+
+    def to(self, device) -> "Int4Weight":
+        return Int4Weight(self.words.to(device), self.scale.to(device), None if self.zero is None else self.zero.to(device),
+                          self.n, self.k, self.group)
+
+    def codes(self) -> torch.Tensor:
+        """uint8 [N, K]."""
+        nt, ks = self.words.shape[:2]
+        sh = torch.tensor([4 * (j >> 1) + 16 * (j & 1) for j in range(8)], dtype=torch.int32, device=self.words.device)
+        c = ((self.words[..., None] >> sh) & 15).to(torch.uint8)                   # [nt, ks, 64, 4, 8]
+        c = c.view(nt, ks, 4, 16, 4, 8).permute(0, 3, 1, 4, 2, 5)                  # nt, r, ks, i, g, j
+        return c.reshape(nt * 16, ks * 128)[: self.n, : self.k].contiguous()
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """[N, K]."""
+        c = self.codes().to(dtype).view(self.n, self.k // self.group, self.group)
+        z = 8.0 if self.zero is None else self.zero[:, : self.n].t().to(dtype)[..., None]
+        return ((c - z) * self.scale[:, : self.n].t().to(dtype)[..., None]).reshape(self.n, self.k)
+
+
+def pack_int4(packed: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None) -> Int4Weight:
+    """packed: uint8 [N, K / 2], feature 2 j in the low and 2 j + 1 in the high four bits of byte j; scale: [N, K / G] bf16 or
+    fp16; zero: uint8 [N, K / G] or None (8)."""
+    if packed.dim() != 2 or packed.dtype != torch.uint8 or scale.dim() != 2 or scale.shape[0] != packed.shape[0]:
+        raise ValueError("packed is uint8 [N, K / 2], scale [N, K / G]")
+    N, K = packed.shape[0], 2 * packed.shape[1]
+    groups = scale.shape[1]
+    G = K // groups if groups else 0
+    if N == 0 or G not in GROUPS or G * groups != K:
+        raise ValueError("K is a multiple of the group size, which is 32, 64 or 128")
+    if scale.dtype not in _DTYPES:
+        raise ValueError("scales are bf16 or fp16")
+    if zero is not None and (zero.shape != scale.shape or zero.dtype != torch.uint8):
+        raise ValueError("zero is uint8 of the scales' shape")
+    nt, ks = (N + 15) // 16, (K + 127) // 128
+    p = torch.zeros((nt * 16, ks * 64), dtype=torch.uint8, device=packed.device)
+    p[:N, : K // 2] = packed
+    # byte m of a word's four holds features (2 m, 2 m + 1): low nibbles to bits 4 m, high ones to 16 + 4 m
+    p = p.view(nt, 16, ks, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)                      # nt, ks, g, r, i, byte
+    lo, hi = p & 15, p >> 4
+    by = torch.stack((lo[..., 0] | (lo[..., 1] << 4), lo[..., 2] | (lo[..., 3] << 4),
+                      hi[..., 0] | (hi[..., 1] << 4), hi[..., 2] | (hi[..., 3] << 4)), -1).contiguous()
+    words = by.view(torch.int32).reshape(nt, ks, 64, 4)
+    pad = lambda t: torch.nn.functional.pad(t.t(), (0, nt * 16 - N)).contiguous()  # noqa: E731
+    return Int4Weight(words, pad(scale), None if zero is None else pad(zero), N, K, G)
+
+
+def quantize_int4(weight: torch.Tensor, group: int = 128, symmetric: bool = True,
+                  scale_dtype: torch.dtype = torch.bfloat16) -> Int4Weight:
+    """Round-to-nearest codes of a float weight [N, K].  Symmetric: zero 8, the scale as small as -8 .. 7 allow; otherwise
+    the group's range (with 0 in it) on 0 .. 15.  Codes are taken with the scale as it is stored."""
+    if weight.dim() != 2 or group not in GROUPS or weight.shape[1] % group != 0:
+        raise ValueError("weight is [N, K] with K a multiple of the group size 32, 64 or 128")
+    N, K = weight.shape
+    w = weight.detach().float().view(N, K // group, group)
+    hi, lo = w.amax(-1).clamp(min=0.0), w.amin(-1).clamp(max=0.0)
+    s = torch.maximum(hi / 7.0, -lo / 8.0) if symmetric else (hi - lo) / 15.0
+    s = torch.where(s > 0, s, torch.ones_like(s)).to(scale_dtype)
+    sf = s.float()
+    z = torch.full_like(sf, 8.0) if symmetric else (-lo / sf).round().clamp(0, 15)
+    c = ((w / sf[..., None]).round() + z[..., None]).clamp(0, 15).to(torch.uint8).view(N, K)
+    return pack_int4(c[:, 0::2] | (c[:, 1::2] << 4), s, None if symmetric else z.to(torch.uint8))
+
+
+def linear_int4_reference(x, w: Int4Weight, bias=None, act: str = "none", res=None) -> torch.Tensor:
+    y = x.float() @ w.dequantize().t()
+    if bias is not None:
+        y = y + bias.float()
+    if res is not None:
+        y = y + res.float()
+    return _act_ref(y, act)
+
+
+def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None, *, act: str = "none",
+                res: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = act(x @ W^T + bias (+ res)) in x's type.  x: [..., K] bf16 or fp16, bias: fp32 [N], res: [..., N] of x's type;
+    act: none, relu, gelu.  Products are exact and summed in fp32, rounded once."""
+    if act not in _ACTS:
+        raise ValueError("act is none, relu or gelu")
+    N, K = w.n, w.k
+    if x.dim() == 0 or x.shape[-1] != K or x.dtype not in _DTYPES:
+        raise ValueError("x is [..., K] bf16 or fp16")
+    if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or bias.stride(0) != 1):
+        raise ValueError("bias is fp32 [N]")
+    if res is not None and (res.shape[:-1] != x.shape[:-1] or res.shape[-1] != N or res.dtype != x.dtype):
+        raise ValueError("res is [..., N] of x's type")
+    dev = x.device
+    if w.words.device != dev or (bias is not None and bias.device != dev) or (res is not None and res.device != dev):
+        raise ValueError("all tensors live on one device")
+    if not x.is_cuda:
+        return linear_int4_reference(x, w, bias, act, res).to(x.dtype)
+    with _loader.device_of(x):
+        x2 = x if x.dim() == 2 else x.reshape(-1, K)
+        if x2.stride(1) != 1 or x2.stride(0) % 8 != 0 or x2.data_ptr() % 16 != 0:
+            x2 = x2.contiguous() if not x2.is_contiguous() else x2.clone()      # rows the kernel can load 16 bytes at a time
+        r2 = None
+        if res is not None:
+            r2 = res if res.dim() == 2 else res.reshape(-1, N)
+            if r2.stride(1) != 1:
+                r2 = r2.contiguous()
+        M = x2.shape[0]
+        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+        rc = _loader.lib().dlamd_int4_linear(
+            x2.data_ptr(), x2.stride(0), w.words.data_ptr(), w.scale.data_ptr(), 0 if w.zero is None else w.zero.data_ptr(),
+            0 if bias is None else bias.data_ptr(), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
+            y.data_ptr(), M, N, K, w.group, _ACTS[act], _DTYPES[x.dtype], _DTYPES[w.scale.dtype], _loader.raw_stream(dev))
+    _loader.check(rc, "dlamd_int4_linear")
+    return y

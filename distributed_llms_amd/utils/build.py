@@ -53,6 +53,10 @@ HIP_FLAGS = [
     # some of their encodings have produced silently wrong values on this hardware pool
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
+# Kernels whose results depend on infinities, NaN or signed borders (masked softmax rows, comparisons of probabilities)
+# are compiled without -ffast-math; a * b + c still becomes one fma.
+PRECISE_FLAGS = ["-fno-fast-math", "-ffp-contract=fast"]
+PRECISE_SOURCES = ("paged_append.hip", "paged_attention.hip", "draft_verify.hip", "int4_linear.hip")
 CXX_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-pthread"]
 
 
@@ -95,7 +99,8 @@ def _compile_objects(srcs: Sequence[Path], compiler: str, flags: List[str], jobs
     for s in srcs:
         o = OBJ_DIR / (s.parent.name + "_" + s.stem + ".o")
         objs.append(o)
-        cmds.append([compiler, *flags, "-c", str(s), "-o", str(o)])
+        extra = PRECISE_FLAGS if s.name in PRECISE_SOURCES else []
+        cmds.append([compiler, *flags, *extra, "-c", str(s), "-o", str(o)])
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
         list(ex.map(_run, cmds))
     return objs
@@ -106,7 +111,7 @@ def build_kernels(force: bool = False, jobs: int = 8, verbose: bool = False) -> 
     srcs = sorted((CSRC / "kernels").glob("*.hip"))
     hdrs = sorted((CSRC / "kernels").glob("*.h"))
     out = LIB_DIR / "libdlamd_kernels.so"
-    digest = _sha(list(srcs) + list(hdrs), " ".join(HIP_FLAGS))
+    digest = _sha(list(srcs) + list(hdrs), " ".join([*HIP_FLAGS, *PRECISE_FLAGS, *PRECISE_SOURCES]))
     if not force and _up_to_date("kernels", digest, out):
         return out
     if not srcs:

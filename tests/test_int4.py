@@ -1,0 +1,179 @@
+"""Linear layers with 4-bit weights, against plain 64-bit products."""
+import math
+
+import pytest
+import torch
+
+from distributed_llms_amd.ops import int4 as Q
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def layer(seed, n, k, group, zero, sdt):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    codes[0, : min(k, 16)] = torch.arange(16, dtype=torch.uint8)[: min(k, 16)]
+    scale = ((torch.rand(n, k // group, generator=g) + 0.1) * (0.3 / math.sqrt(k))).to(sdt)
+    z = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.uint8) if zero else None
+    return codes, scale, z, Q.pack_int4(codes[:, 0::2] | (codes[:, 1::2] << 4), scale, z)
+
+
+def weights64(codes, scale, z, group):
+    zz = 8.0 if z is None else z.double().repeat_interleave(group, 1)
+    return (codes.double() - zz) * scale.double().repeat_interleave(group, 1)
+
+
+def act64(y, act):
+    if act == "relu":
+        return y.clamp(min=0)
+    return 0.5 * y * torch.special.erfc(-y / math.sqrt(2)) if act == "gelu" else y
+
+
+def check(got, x, codes, scale, z, group, bias, act, res):
+    """Tolerance: half a step of the output's type (gelu's slope is at most 1.13), and the fp32 sums.  Codes enter the
+    products with an offset of 128 (bf16) or 1024 (fp16) that is taken out again, so a group's sum of |x| (offset + 16) s
+    carries up to 16 roundings of 2^-24 (a matrix instruction adds its 32 products in a tree, a group is at most four of
+    them, then the offset and the scale); bias, residual and the join of partial sums add a few more of the result."""
+    w = weights64(codes, scale, z, group)
+    lead = x.shape[:-1]
+    x2 = x.double().reshape(-1, x.shape[-1])
+    y = x2 @ w.t()
+    y = y if bias is None else y + bias.double()
+    y = y if res is None else y + res.double().reshape(y.shape)
+    ref = act64(y, act)
+    off = 128 if x.dtype == torch.bfloat16 else 1024
+    mass = x2.abs() @ scale.double().repeat_interleave(group, 1).t()
+    tol = torch.finfo(x.dtype).eps / 2 * ref.abs() + 2.0 ** -24 * (16 * (off + 16) * mass + 64 * y.abs() + 64) * 1.13
+    if x.dtype == torch.float16:
+        tol += 2.0 ** -25            # below 2^-14 a fp16 step is 2^-24
+    assert got.dtype == x.dtype and got.shape == (*lead, codes.shape[0])
+    err = (got.double().reshape(y.shape) - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+CASES = [  # rows, n, k, group, zero, act, bias, res, x type, scale type
+    (1, 1, 32, 32, False, "none", False, False, "bf16", "bf16"),
+    (1, 4096, 1024, 64, False, "gelu", True, False, "bf16", "bf16"),
+    (5, 301, 1024, 128, True, "none", True, False, "bf16", "fp16"),
+    (16, 33, 96, 32, True, "relu", False, True, "fp16", "fp16"),
+    (17, 1000, 448, 64, False, "none", True, True, "fp16", "bf16"),
+    (2, 17, 4096, 128, True, "gelu", True, True, "bf16", "bf16"),
+    (64, 256, 256, 128, False, "none", False, False, "bf16", "bf16"),
+    (65, 130, 160, 32, True, "none", True, False, "bf16", "bf16"),
+    (150, 48, 640, 128, False, "relu", True, True, "fp16", "fp16"),
+    (3, 5000, 8192, 128, True, "none", True, False, "fp16", "fp16"),
+    (40, 777, 2080, 32, True, "gelu", True, True, "bf16", "bf16"),
+]
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def to(dev, *xs):
+    return [None if x is None else x.to(dev) for x in xs]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_matches_plain(dev, i):
+    rows, n, k, group, zero, act, has_bias, has_res, dt, sdt = CASES[i]
+    codes, scale, z, w = layer(i, n, k, group, zero, DTYPES[sdt])
+    g = torch.Generator().manual_seed(50 + i)
+    x = torch.randn(rows, k, generator=g).to(DTYPES[dt])
+    bias = torch.randn(n, generator=g) if has_bias else None
+    res = torch.randn(rows, n, generator=g).to(DTYPES[dt]) if has_res else None
+    xd, bd, rd, wd = *to(dev, x, bias, res), w.to(dev)
+    got = Q.linear_int4(xd, wd, bd, act=act, res=rd)
+    check(got.cpu(), x, codes, scale, z, group, bias, act, res)
+    assert torch.equal(Q.linear_int4(xd, wd, bd, act=act, res=rd), got)       # again: the same bits
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_one_feature_at_a_time(dev):
+    """x picks single weights: every code of every row comes back from its own place."""
+    for k, group in ((160, 32), (256, 128)):
+        codes, scale, z, w = layer(k, 50, k, group, True, torch.bfloat16)
+        scale.fill_(0.5)
+        w.scale.fill_(0.5)
+        got = Q.linear_int4(torch.eye(k, dtype=torch.bfloat16).to(dev), w.to(dev)).cpu()
+        assert torch.equal(got.double().t(), weights64(codes, scale, z, group))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_strided_rows_and_leading_dimensions(dev):
+    codes, scale, z, w = layer(1, 70, 128, 64, False, torch.bfloat16)
+    g = torch.Generator().manual_seed(2)
+    big = torch.randn(6, 3, 300, generator=g).to(torch.bfloat16)
+    res = torch.randn(6, 3, 90, generator=g).to(torch.bfloat16)
+    w = w.to(dev)
+    for sl in (slice(0, 128), slice(8, 136), slice(3, 131)):
+        x, r = big[..., sl], res[..., 5:75]
+        bd, rd = big.to(dev), res.to(dev)
+        check(Q.linear_int4(bd[..., sl], w, res=rd[..., 5:75]).cpu(), x, codes, scale, z, 64, None, "none", r)
+        check(Q.linear_int4(bd[:, 0, sl], w, res=rd[:, 0, 5:75]).cpu(), x[:, 0], codes, scale, z, 64, None, "none", r[:, 0])
+    x = big[0, :, ::2][:, :128]
+    check(Q.linear_int4(big.to(dev)[0, :, ::2][:, :128], w).cpu(), x, codes, scale, z, 64, None, "none", None)
+    x1 = big[0, 0, :128]
+    check(Q.linear_int4(x1.to(dev), w).cpu(), x1, codes, scale, z, 64, None, "none", None)
+    assert Q.linear_int4(big[:0, 0, :128].to(dev), w).shape == (0, 70)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_row_with_nan_or_infinity_stays_alone(dev):
+    codes, scale, z, w = layer(4, 40, 256, 64, True, torch.bfloat16)
+    x = torch.randn(20, 256, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    bad = x.clone()
+    bad[3, 7], bad[17, 100] = float("nan"), float("inf")
+    got = Q.linear_int4(bad.to(dev), w.to(dev)).cpu()
+    assert not torch.isfinite(got[3]).any() and not torch.isfinite(got[17]).all()
+    keep = [i for i in range(20) if i not in (3, 17)]
+    check(got[keep], x[keep], codes, scale, z, 64, None, "none", None)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("group", Q.GROUPS)
+def test_quantize_is_round_to_nearest(group, symmetric):
+    g = torch.Generator().manual_seed(group)
+    w = torch.randn(37, 4 * group, generator=g) * 0.05
+    w[3, :group] = 0.0
+    w[4, :group] = w[4, :group].abs() + 0.1
+    q = Q.quantize_int4(w, group, symmetric)
+    d = q.dequantize(torch.float64)
+    assert torch.equal(d, weights64(q.codes(), q.scale[:, :37].t(), None if q.zero is None else q.zero[:, :37].t(), group))
+    s = q.scale[:, :37].t().double().repeat_interleave(group, 1)
+    # half a step of the grid; at the ends of the range the stored (bf16) scale and a rounded zero shift it by up to
+    # 8 steps 2^-8 + 1/2 step (15 steps 2^-8 + 1/2)
+    slack = 8 * 2.0 ** -8 if symmetric else 15 * 2.0 ** -8 + 0.5
+    assert bool(((d - w.double()).abs() <= s * (0.5 + slack)).all())
+    inside = (q.codes() > 0) & (q.codes() < 15)
+    assert bool(((d - w.double()).abs() <= s * 0.5001)[inside].all())
+    assert bool((d[3, :group] == 0).all())
+
+
+REFUSED = {
+    "K of another layer": lambda c: c.update(x=c["x"][:, :32]),
+    "fp32 rows": lambda c: c.update(x=c["x"].float()),
+    "an unknown activation": lambda c: c.update(act="tanh"),
+    "bf16 bias": lambda c: c.update(bias=torch.zeros(40, dtype=torch.bfloat16)),
+    "short bias": lambda c: c.update(bias=torch.zeros(39)),
+    "res of another type": lambda c: c.update(res=torch.zeros(2, 40)),
+    "res of another shape": lambda c: c.update(res=torch.zeros(3, 40, dtype=torch.bfloat16)),
+}
+
+
+@pytest.mark.parametrize("why", sorted(REFUSED))
+def test_refuses(why):
+    c = dict(x=torch.zeros(2, 64, dtype=torch.bfloat16), w=layer(0, 40, 64, 32, False, torch.bfloat16)[3])
+    REFUSED[why](c)
+    with pytest.raises(ValueError):
+        Q.linear_int4(**c)
+
+
+def test_refuses_to_pack():
+    p, s = torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 2, dtype=torch.bfloat16)
+    Q.pack_int4(p, s)
+    for bad in (dict(packed=p.int()), dict(scale=s.float()), dict(scale=torch.ones(4, 3, dtype=torch.bfloat16)), dict(scale=s[:3]),
+                dict(zero=torch.zeros(4, 2)), dict(scale=torch.ones(4, 8, dtype=torch.bfloat16)), dict(packed=p[:0], scale=s[:0])):
+        with pytest.raises(ValueError):
+            Q.pack_int4(**{"packed": p, "scale": s, **bad})
+    for bad in (dict(group=48), dict(weight=torch.zeros(4, 100)), dict(weight=torch.zeros(4))):
+        with pytest.raises(ValueError):
+            Q.quantize_int4(**{"weight": torch.zeros(4, 128), "group": 64, **bad})

@@ -1,0 +1,441 @@
+"""Paged key / value cache: append with rotation and attention of new tokens, against plain 64-bit implementations."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from distributed_llms_amd.ops import paged as P
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def cache(pages, page, hkv, D, dt, g, layout="plain"):
+    """k_pages, v_pages; layout "joint": slices of one [pages, 2, page, ...] buffer, "heads": heads outside the slots."""
+    if layout == "joint":
+        kv = torch.randn(pages, 2, page, hkv, D, generator=g).to(dt)
+        return kv[:, 0], kv[:, 1]
+    if layout == "heads":
+        kv = torch.randn(2, pages, hkv, page, D, generator=g).to(dt)
+        return kv[0].transpose(1, 2), kv[1].transpose(1, 2)
+    return tuple(torch.randn(pages, page, hkv, D, generator=g).to(dt) for _ in range(2))
+
+
+def tables(need, page, g, extra=2, width=None):
+    """Page table of random distinct pages for sequences of ``need`` tokens, -1 behind; (table, number of pages)."""
+    counts = [-(-n // page) for n in need]
+    total = sum(counts) + extra
+    perm = torch.randperm(total, generator=g).to(torch.int32)
+    t = torch.full((len(need), width or max([1] + counts)), -1, dtype=torch.int32)
+    at = 0
+    for b, c in enumerate(counts):
+        t[b, :c] = perm[at : at + c]
+        at += c
+    return t, total
+
+
+def gpu(*xs):
+    return [None if x is None else x.cuda() for x in xs]
+
+
+def on_gpu_with_strides(x):
+    """A copy on the GPU with the strides of ``x`` (``.cuda()`` keeps them only for dense tensors)."""
+    y = torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device="cuda")
+    return y.copy_(x)
+
+
+# ---------------------------------------------------------------------------------------------- append
+def append_case(seed, need_new, kept, page, hkv, hq, D, rot, dt, interleaved, ragged, layout="plain", behind=0):
+    g = torch.Generator().manual_seed(seed)
+    B = len(kept)
+    T = sum(need_new) + behind
+    table, pages = tables([max(k, 0) + n for k, n in zip(kept, need_new)], page, g)
+    kp, vp = cache(pages, page, hkv, D, dt, g, layout)
+    qkv = torch.randn(T, hq + 2 * hkv, D, generator=g).to(dt)
+    q, k, v = qkv[:, :hq], qkv[:, hq : hq + hkv], qkv[:, hq + hkv :]
+    lens = torch.tensor(kept, dtype=torch.int32)
+    starts = torch.tensor([sum(need_new[:b]) for b in range(B + 1)], dtype=torch.int32) if ragged else None
+    cos, sin = P.rope_tables(table.shape[1] * page, rot) if rot else (None, None)
+    return dict(k=k, v=v, k_pages=kp, v_pages=vp, table=table, lens=lens, q=q if hq else None, cos=cos, sin=sin, starts=starts,
+                interleaved=interleaved)
+
+
+def close_half_step(got, ref, dt):
+    """One rounding (half a step of ``dt``) of fp32 maths whose own error is a few fp32 steps of the operands (|x| < 8)."""
+    err = (got.double() - ref.double()).abs()
+    tol = torch.finfo(dt).eps / 2 * ref.double().abs() + 32 * 2.0 ** -24
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+def rotate64(x, pos, rot, interleaved):
+    """Rotation as complex numbers, angles from the position in 64 bits."""
+    x = x.double()
+    if rot == 0:
+        return x
+    w = torch.polar(torch.ones(rot // 2, dtype=torch.float64), pos * 10000.0 ** (-torch.arange(rot // 2, dtype=torch.float64) * 2 / rot))
+    r = x[..., :rot]
+    if interleaved:
+        z = torch.view_as_complex(r.reshape(*r.shape[:-1], rot // 2, 2).contiguous()) * w
+        y = torch.view_as_real(z).reshape(r.shape)
+    else:
+        z = torch.complex(r[..., : rot // 2].contiguous(), r[..., rot // 2 :].contiguous()) * w
+        y = torch.cat((z.real, z.imag), -1)
+    return torch.cat((y, x[..., rot:]), -1)
+
+
+def check_append(c, got_k, got_v, got_q, rot):
+    """Expected cache and queries token by token from the definition."""
+    B, (pages, page) = len(c["lens"]), c["k_pages"].shape[:2]
+    T = c["k"].shape[0]
+    dt = c["k"].dtype
+    kp, vp = c["k_pages"].double().clone(), c["v_pages"].double().clone()
+    qo = torch.zeros(c["q"].shape, dtype=torch.float64) if c["q"] is not None else None
+    starts = c["starts"].tolist() if c["starts"] is not None else [T // B * b for b in range(B + 1)]
+    written = torch.zeros(pages, page, dtype=torch.bool)
+    for b in range(B):
+        for t in range(starts[b], min(starts[b + 1], T)):
+            pos = int(c["lens"][b]) + t - starts[b]
+            if int(c["lens"][b]) < 0 or pos >= c["table"].shape[1] * page:
+                continue
+            if qo is not None:
+                qo[t] = rotate64(c["q"][t], pos, rot, c["interleaved"])
+            pid = int(c["table"][b, pos // page])
+            if 0 <= pid < pages:
+                kp[pid, pos % page] = rotate64(c["k"][t], pos, rot, c["interleaved"])
+                vp[pid, pos % page] = c["v"][t].double()
+                written[pid, pos % page] = True
+    assert torch.equal(got_v.double(), vp)
+    assert torch.equal(got_k.double()[~written], kp[~written])          # what was there stays, bit for bit
+    # angles of far positions: the table holds them to half a fp32 step, so a rotated value is off by |x| 2^-24 more
+    close_half_step(got_k, kp, dt)
+    if qo is not None:
+        close_half_step(got_q, qo, dt)
+
+
+APPEND = [
+    # need_new, kept, page, hkv, hq, D, rot, dtype, interleaved, ragged, layout, behind
+    ([1], [0], 16, 1, 0, 64, 0, "bf16", False, False, "plain", 0),
+    ([1] * 5, [0, 15, 16, 31, 200], 16, 16, 0, 64, 0, "bf16", False, False, "plain", 0),
+    ([5] * 3, [0, 13, 63], 64, 8, 32, 128, 128, "fp16", False, False, "joint", 0),
+    ([4] * 4, [-1, 3, -7, 0], 16, 2, 4, 64, 32, "bf16", True, False, "plain", 0),
+    ([7, 0, 33, 1, 0], [0, 5, 40, 100, 3], 48, 2, 6, 64, 16, "bf16", False, True, "heads", 9),
+    ([0, 0, 3], [0, 0, 0], 16, 1, 1, 128, 64, "fp16", True, True, "plain", 0),
+    ([130, 1, 77], [9000, 0, 31], 128, 3, 3, 128, 128, "bf16", True, True, "joint", 64),
+    ([2] * 70, [i * 3 for i in range(70)], 8, 1, 2, 72, 48, "bf16", False, True, "plain", 3),
+    ([3] * 200, [(i * 37) % 90 for i in range(200)], 5, 2, 2, 64, 64, "fp16", False, True, "plain", 0),
+]
+
+
+@pytest.mark.parametrize("case", range(len(APPEND)))
+def test_append_oracle(case):
+    n, kept, page, hkv, hq, D, rot, dt, il, ragged, layout, behind = APPEND[case]
+    c = append_case(case, n, kept, page, hkv, hq, D, rot, DTYPES[dt], il, ragged, layout, behind)
+    kp, vp = c["k_pages"].clone(), c["v_pages"].clone()
+    qo = P.paged_append(**{**c, "k_pages": kp, "v_pages": vp})
+    check_append(c, kp, vp, qo, rot)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(APPEND)))
+def test_append_kernel(case):
+    n, kept, page, hkv, hq, D, rot, dt, il, ragged, layout, behind = APPEND[case]
+    c = append_case(case, n, kept, page, hkv, hq, D, rot, DTYPES[dt], il, ragged, layout, behind)
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    full = torch.empty((c["k"].shape[0], hq + 2 * hkv, D), dtype=DTYPES[dt], device="cuda")       # slices of one projection
+    full[:, hq : hq + hkv], full[:, hq + hkv :] = c["k"].cuda(), c["v"].cuda()
+    if hq:
+        full[:, :hq] = c["q"].cuda()
+        d["q"] = full[:, :hq]
+    d["k"], d["v"] = full[:, hq : hq + hkv], full[:, hq + hkv :]
+    d["k_pages"], d["v_pages"] = on_gpu_with_strides(c["k_pages"]), on_gpu_with_strides(c["v_pages"])
+    before = full.clone()
+    qo = P.paged_append(**d)
+    assert torch.equal(full, before)
+    check_append(c, d["k_pages"].cpu(), d["v_pages"].cpu(), None if qo is None else qo.cpu(), rot)
+
+
+def bad_table_case():
+    c = append_case(3, [4] * 4, [0, 14, 30, 2], 16, 2, 2, 64, 64, torch.bfloat16, False, False)
+    c["table"] = torch.tensor([[-1, 0, 0], [0, 1 << 30, 0], [1, 2, -(1 << 31)], [c["k_pages"].shape[0], 0, 0]], dtype=torch.int32)
+    c["cos"], c["sin"] = P.rope_tables(48, 64)
+    return c
+
+
+def test_append_to_missing_pages_writes_nothing():
+    c = bad_table_case()
+    kp, vp = c["k_pages"].clone(), c["v_pages"].clone()
+    qo = P.paged_append(**{**c, "k_pages": kp, "v_pages": vp})
+    check_append(c, kp, vp, qo, 64)
+
+
+@pytest.mark.gpu
+def test_append_kernel_to_missing_pages_writes_nothing():
+    c = bad_table_case()
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    qo = P.paged_append(**d)
+    check_append(c, d["k_pages"].cpu(), d["v_pages"].cpu(), qo.cpu(), 64)
+
+
+def test_rope_tables_are_exact_at_far_positions():
+    cos, sin = P.rope_tables(200001, 16)
+    ang = 200000 * 10000.0 ** (-2.0 / 16)
+    assert abs(float(cos[200000, 1]) - math.cos(ang)) <= 2.0 ** -24 and abs(float(sin[200000, 1]) - math.sin(ang)) <= 2.0 ** -24
+
+
+# ---------------------------------------------------------------------------------------------- attention
+def att_case(seed, kept, n, page, hq, hkv, D, dt, causal, layout="plain", qscale=1.5):
+    g = torch.Generator().manual_seed(seed)
+    need = [max(k, 0) + (n if causal and k >= 0 else 0) for k in kept]
+    table, pages = tables(need, page, g)
+    kp, vp = cache(pages, page, hkv, D, dt, g, layout)
+    # slots nobody has written hold NaN and infinities
+    used = torch.zeros(pages, page, dtype=torch.bool)
+    for b, m in enumerate(need):
+        for p in range(m):
+            used[int(table[b, p // page]), p % page] = True
+    kp[~used] = float("nan")
+    vp[~used] = float("inf")
+    q = (torch.randn(len(kept), n, hq, D, generator=g) * qscale).to(dt)
+    return dict(q=q, k_pages=kp, v_pages=vp, table=table, lens=torch.tensor(kept, dtype=torch.int32), causal=causal)
+
+
+def att_tolerance(c, ref):
+    """Half a step of the output's type, plus the fp32 maths: scores |s| < 64 carry 2^-24 |s| (D + 2) in the worst case of
+    their sum, which the exponential turns into that relative error; the weights are kept to 2^-16."""
+    vmax = c["v_pages"].double().nan_to_num(0, 0, 0).abs().max()
+    return torch.finfo(c["q"].dtype).eps / 2 * ref.abs() + float(vmax) * 2.0 ** -13
+
+
+def check_attention(c, o, lse):
+    ref, ref_lse = P.paged_attention_reference(**c, dtype=torch.float64)
+    assert o.dtype == c["q"].dtype and o.shape == c["q"].shape and lse.dtype == torch.float32
+    err = (o.double() - ref).abs()
+    assert bool((err <= att_tolerance(c, ref)).all()), float(err.max())
+    empty = torch.isinf(ref_lse)
+    assert torch.equal(torch.isinf(lse.double()), empty) and bool((lse[empty] < 0).all()) and bool((o[empty] == 0).all())
+    assert bool(((lse.double() - ref_lse).abs()[~empty] <= 2.0 ** -24 * 130 * 64).all())
+
+
+ATT = [
+    # kept, n, page, hq, hkv, D, dtype, causal, layout
+    ([0], 1, 16, 1, 1, 64, "bf16", True, "plain"),
+    ([0, 1, 30, 31, 32, 127], 1, 16, 4, 4, 64, "bf16", True, "plain"),
+    ([0, -1, 5, 64], 1, 32, 2, 2, 64, "bf16", False, "joint"),
+    ([577] * 3, 1, 32, 16, 16, 64, "bf16", False, "plain"),
+    ([100, 0, 47, 48, 1000], 5, 48, 32, 4, 128, "fp16", True, "joint"),
+    ([3, 2500], 3, 16, 6, 2, 128, "bf16", True, "heads"),
+    ([4999], 1, 64, 32, 8, 128, "bf16", True, "plain"),
+    ([20011, 7], 2, 80, 4, 1, 64, "fp16", True, "plain"),
+    ([17, 300], 16, 16, 24, 2, 128, "bf16", True, "plain"),
+    ([33, 0, 600], 9, 256, 7, 1, 64, "fp16", False, "heads"),
+    ([9] * 70, 2, 16, 4, 2, 64, "bf16", True, "plain"),
+    ([700], 40, 32, 5, 1, 64, "bf16", True, "plain"),
+]
+
+
+@pytest.mark.parametrize("case", [0, 2, 4, 9])
+def test_attention_oracle_against_dense_attention(case):
+    kept, n, page, hq, hkv, D, dt, causal, layout = ATT[case]
+    c = att_case(case, kept, n, page, hq, hkv, D, DTYPES[dt], causal, layout)
+    o, lse = P.paged_attention(**c, return_lse=True)
+    check_attention(c, o, lse)
+    for b, m in enumerate(kept):
+        for i in range(n):
+            seen = max(m, 0) + (i + 1 if causal and m >= 0 else 0)
+            if seen == 0:
+                continue
+            pos = torch.arange(seen)
+            pid = c["table"][b].long()[pos // page]
+            k, v = (x[pid, pos % page].double().repeat_interleave(hq // hkv, 1).transpose(0, 1) for x in (c["k_pages"], c["v_pages"]))
+            ref = F.scaled_dot_product_attention(c["q"][b, i].double()[:, None], k, v)[:, 0]
+            assert bool(((o[b, i].double() - ref).abs() <= att_tolerance(c, ref)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(ATT)))
+def test_attention_kernel(case):
+    kept, n, page, hq, hkv, D, dt, causal, layout = ATT[case]
+    c = att_case(case, kept, n, page, hq, hkv, D, DTYPES[dt], causal, layout)
+    d = {x: on_gpu_with_strides(y) if torch.is_tensor(y) else y for x, y in c.items()}
+    o, lse = P.paged_attention(**d, return_lse=True)
+    check_attention(c, o.cpu(), lse.cpu())
+    assert torch.equal(P.paged_attention(**d), o)                     # without the log-sum-exp, and again: the same bits
+
+
+def missing_pages_case():
+    c = att_case(11, [100, 60, 33], 2, 16, 8, 2, 64, torch.bfloat16, True)
+    c["table"][0, 2] = -1                       # a hole
+    c["table"][1] = torch.tensor(c["k_pages"].shape[0], dtype=torch.int32)      # no page at all
+    c["table"][2, 0] = 1 << 30
+    return c
+
+
+def test_attention_oracle_skips_missing_pages():
+    c = missing_pages_case()
+    o, lse = P.paged_attention(**c, return_lse=True)
+    check_attention(c, o, lse)
+    assert bool((o[1] == 0).all()) and not bool((o[0] == 0).all())
+
+
+@pytest.mark.gpu
+def test_attention_kernel_skips_missing_pages():
+    c = missing_pages_case()
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o, lse = P.paged_attention(**d, return_lse=True)
+    check_attention(c, o.cpu(), lse.cpu())
+
+
+def peaked_case():
+    """Scores from -600 to 600: one key takes everything, and it lies near the end, in the middle or in front."""
+    c = att_case(5, [400, 390, 380], 1, 16, 4, 2, 64, torch.bfloat16, True, qscale=1.0)
+    for b, at in enumerate((399, 200, 0)):
+        pid = int(c["table"][b, at // 16])
+        c["k_pages"][pid, at % 16] = (c["q"][b, 0].view(2, 2, 64)[:, 0].float() * 8).to(torch.bfloat16)
+    c["q"] = (c["q"].float() * 8).to(torch.bfloat16)
+    return c
+
+
+@pytest.mark.gpu
+def test_attention_kernel_with_peaked_scores():
+    c = peaked_case()
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o, lse = (x.cpu() for x in P.paged_attention(**d, return_lse=True))
+    ref, ref_lse = P.paged_attention_reference(**c, dtype=torch.float64)
+    assert torch.isfinite(o).all()
+    # scores up to 700 carry 2^-24 * 700 * 66 < 2^-8.5 absolute error in the worst case, as relative error of the weights
+    vmax = float(c["v_pages"].double().nan_to_num(0, 0, 0).abs().max())
+    assert bool(((o.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + vmax * 2.0 ** -8).all())
+    assert bool(((lse.double() - ref_lse).abs() <= 2.0 ** -8).all())
+
+
+@pytest.mark.gpu
+def test_attention_kernel_with_infinite_and_nan_keys_in_sight():
+    """A visible key whose score is -inf weighs nothing; a NaN in a visible value reaches its own row only."""
+    c = att_case(6, [50, 50], 1, 16, 2, 2, 64, torch.bfloat16, True)
+    c["q"] = c["q"].abs() + 0.1
+    c["q"] = c["q"].to(torch.bfloat16)
+    c["k_pages"][int(c["table"][0, 1]), 3] = float("-inf")
+    c["v_pages"][int(c["table"][1, 1]), 3, 0, 5] = float("nan")
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o = P.paged_attention(**d).cpu()
+    ref, _ = P.paged_attention_reference(**c, dtype=torch.float64)
+    assert bool(((o[0].double() - ref[0]).abs() <= att_tolerance(c, ref[0])).all())
+    nan = torch.isnan(o)
+    assert bool(nan[1, 0, 0, 5]) and int(nan.sum()) == 1
+
+
+@pytest.mark.gpu
+def test_attention_kernel_offsets_beyond_32_bits():
+    """A cache of more than 2^31 elements (4.3 GB each of K and V): the sequence's pages lie at both ends."""
+    page, hkv, D = 256, 8, 128
+    pages = (1 << 31) // (page * hkv * D) + 8
+    kp = torch.zeros((pages, page, hkv, D), dtype=torch.bfloat16, device="cuda")
+    vp = torch.zeros_like(kp)
+    g = torch.Generator().manual_seed(9)
+    small_k, small_v = (torch.randn(3, page, hkv, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    where = [pages - 1, 0, pages - 3]
+    for j, pid in enumerate(where):
+        kp[pid], vp[pid] = small_k[j].cuda(), small_v[j].cuda()
+    new_k, new_v = (torch.randn(1, hkv, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    table = torch.tensor([where], dtype=torch.int32)
+    lens = torch.tensor([700], dtype=torch.int32)
+    q = torch.randn(1, 1, 16, D, generator=g).to(torch.bfloat16)
+    P.paged_append(new_k.cuda(), new_v.cuda(), kp, vp, table.cuda(), lens.cuda())
+    o = P.paged_attention(q.cuda(), kp, vp, table.cuda(), lens.cuda()).cpu()
+    small_k[2, 700 - 512], small_v[2, 700 - 512] = new_k[0], new_v[0]
+    c = dict(q=q, k_pages=small_k, v_pages=small_v, table=torch.tensor([[0, 1, 2]], dtype=torch.int32), lens=lens, causal=True)
+    ref, _ = P.paged_attention_reference(**c, dtype=torch.float64)
+    assert bool(((o.double() - ref).abs() <= att_tolerance(c, ref)).all())
+    del kp, vp
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    assert P.paged_attention(z(0, 1, 2, 64), z(1, 16, 2, 64), z(1, 16, 2, 64), i(0, 1), i(0)).shape == (0, 1, 2, 64)
+    assert P.paged_attention(z(2, 0, 2, 64), z(1, 16, 2, 64), z(1, 16, 2, 64), i(2, 1), i(2)).numel() == 0
+    o, lse = P.paged_attention(z(2, 1, 2, 64) + 1, z(1, 16, 2, 64), z(1, 16, 2, 64), i(2, 0), i(2), return_lse=True)
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    o = P.paged_attention(z(2, 1, 2, 64) + 1, z(0, 16, 2, 64), z(0, 16, 2, 64), i(2, 3), i(2) + 9)
+    assert bool((o == 0).all())
+    kp = z(1, 16, 2, 64)
+    assert P.paged_append(z(0, 2, 64), z(0, 2, 64), kp, kp.clone(), i(3, 1), i(3)) is None
+    q = P.paged_append(z(3, 2, 64) + 1, z(3, 2, 64), kp, kp.clone(), i(3, 0), i(3), q=z(3, 2, 64) + 1)
+    assert bool((q == 0).all()) and bool((kp == 0).all())
+
+
+# ---------------------------------------------------------------------------------------------- refusals
+def _append_args():
+    c = append_case(1, [2] * 2, [0, 3], 16, 2, 4, 64, 32, torch.bfloat16, False, False)
+    return c
+
+
+APPEND_REFUSED = {
+    "types differ": lambda c: c.update(k=c["k"].half()),
+    "cache types differ": lambda c: c.update(v_pages=c["v_pages"].half()),
+    "fp32 cache": lambda c: c.update(k_pages=c["k_pages"].float(), v_pages=c["v_pages"].float()),
+    "heads differ": lambda c: c.update(k=c["k"][:, :1], v=c["v"][:, :1]),
+    "not one token count": lambda c: c.update(v=c["v"][:2]),
+    "uneven without starts": lambda c: c.update(k=c["k"][:3], v=c["v"][:3], q=None),
+    "short rotation tables": lambda c: c.update(cos=c["cos"][:5], sin=c["sin"][:5]),
+    "cos without sin": lambda c: c.update(sin=None),
+    "odd rotation": lambda c: c.update(cos=c["cos"][:, :5], sin=c["sin"][:, :5]),
+    "rotation beyond D": lambda c: c.update(cos=torch.zeros(64, 40), sin=torch.zeros(64, 40)),
+    "64-bit lens": lambda c: c.update(lens=c["lens"].long()),
+    "64-bit table": lambda c: c.update(table=c["table"].long()),
+    "lens of another batch": lambda c: c.update(lens=c["lens"][:1]),
+    "starts of another batch": lambda c: c.update(starts=torch.zeros(2, dtype=torch.int32)),
+    "last dimension strided": lambda c: c.update(k=c["k"].transpose(0, 2).contiguous().transpose(0, 2)),
+    "q of another type": lambda c: c.update(q=c["q"].half()),
+    "q of another length": lambda c: c.update(q=c["q"][:2]),
+}
+
+
+@pytest.mark.parametrize("why", sorted(APPEND_REFUSED))
+def test_append_refuses(why):
+    c = _append_args()
+    APPEND_REFUSED[why](c)
+    with pytest.raises(ValueError):
+        P.paged_append(**c)
+
+
+ATT_REFUSED = {
+    "types differ": lambda c: c.update(q=c["q"].half()),
+    "heads no multiple": lambda c: c.update(q=c["q"][:, :, :3]),
+    "page 8": lambda c: c.update(k_pages=c["k_pages"][:, :8], v_pages=c["v_pages"][:, :8]),
+    "D 32": lambda c: c.update(q=c["q"][..., :32], k_pages=c["k_pages"][..., :32], v_pages=c["v_pages"][..., :32]),
+    "D differs": lambda c: c.update(q=c["q"][..., :32]),
+    "table of another batch": lambda c: c.update(table=c["table"][:1], lens=c["lens"][:1]),
+    "64-bit lens": lambda c: c.update(lens=c["lens"].long()),
+    "one query, no n": lambda c: c.update(q=c["q"][:, 0]),
+    "K and V differ": lambda c: c.update(v_pages=c["v_pages"][:1]),
+}
+
+
+@pytest.mark.parametrize("why", sorted(ATT_REFUSED))
+def test_attention_refuses(why):
+    c = att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True)
+    ATT_REFUSED[why](c)
+    with pytest.raises(ValueError):
+        P.paged_attention(**c)
+
+
+@pytest.mark.gpu
+def test_kernels_refuse_what_they_cannot_load():
+    """Misaligned rows (16 bytes at a time) and a misplaced tensor are refused on the host, nothing is launched."""
+    from distributed_llms_amd.ops._loader import KernelLibraryError
+
+    c = att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True)
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    q = torch.zeros(2 * 4 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(2, 1, 4, 64)
+    with pytest.raises(KernelLibraryError):
+        P.paged_attention(**{**d, "q": q})
+    with pytest.raises(ValueError):
+        P.paged_attention(**{**d, "lens": c["lens"]})
+    odd = torch.zeros(2, 2, 65, dtype=torch.bfloat16, device="cuda")[..., :64]
+    with pytest.raises(KernelLibraryError):
+        P.paged_append(odd, odd, d["k_pages"], d["v_pages"], d["table"], d["lens"])
+    with pytest.raises(ValueError):
+        P.paged_append(odd.cpu(), odd.cpu(), d["k_pages"], d["v_pages"], d["table"], d["lens"])
