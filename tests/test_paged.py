@@ -324,6 +324,44 @@ def test_attention_kernel_with_infinite_and_nan_keys_in_sight():
     assert bool(nan[1, 0, 0, 5]) and int(nan.sum()) == 1
 
 
+def odd_values_case(dt):
+    """NaN and infinities in the values of the newest tokens: rows of earlier tokens do not see them."""
+    c = att_case(13, [63, 90, 400], 6, 16, 16, 2, 128, dt, True)
+    for b, (i, d, x) in enumerate(((1, 0, float("nan")), (5, 127, float("inf")), (3, 64, float("-inf")))):
+        pos = int(c["lens"][b]) + i
+        c["v_pages"][int(c["table"][b, pos // 16]), pos % 16, :, d] = x
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_attention_kernel_keeps_odd_values_from_rows_that_do_not_see_them(dt):
+    c = odd_values_case(DTYPES[dt])
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o = P.paged_attention(**d).cpu()
+    ref, _ = P.paged_attention_reference(**c, dtype=torch.float64)
+    for b, (i, dim) in enumerate(((1, 0), (5, 127), (3, 64))):
+        assert torch.isfinite(o[b, :i]).all() and not torch.isfinite(o[b, i:, :, dim]).any()
+        assert torch.isfinite(o[b, i:].double()).sum() == torch.isfinite(ref[b, i:]).sum()
+    ok = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(o), torch.isnan(ref)) and torch.equal(o[~ok].isinf(), ref[~ok].isinf())
+    vmax = float(c["v_pages"].double().nan_to_num(0, 0, 0).abs().max())
+    assert bool(((o.double() - ref).abs()[ok] <= torch.finfo(DTYPES[dt]).eps / 2 * ref.abs()[ok] + vmax * 2.0 ** -13).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [4, 6, 7, 8])
+@pytest.mark.parametrize("splits,chunk", [(2, 128), (3, 384), (40, 128), (1, 128)])
+def test_attention_kernel_splits(case, splits, chunk, monkeypatch):
+    """Any split gives the result, also one whose last chunk takes more than its share."""
+    kept, n, page, hq, hkv, D, dt, causal, layout = ATT[case]
+    c = att_case(case, kept, n, page, hq, hkv, D, DTYPES[dt], causal, layout)
+    d = {x: on_gpu_with_strides(y) if torch.is_tensor(y) else y for x, y in c.items()}
+    monkeypatch.setattr(P, "_split", lambda units, bound: (splits, chunk))
+    o, lse = P.paged_attention(**d, return_lse=True)
+    check_attention(c, o.cpu(), lse.cpu())
+
+
 @pytest.mark.gpu
 def test_attention_kernel_offsets_beyond_32_bits():
     """A cache of more than 2^31 elements (4.3 GB each of K and V): the sequence's pages lie at both ends."""
