@@ -6,6 +6,15 @@
 // so a lane's 16-byte load holds its operands of four instructions and a wave's load is 1 KB in one piece.  Inside a word
 // code 2 p lies in bits 4 p and code 2 p + 1 in bits 16 + 4 p: (word >> 4 p) & 0x000f000f is a pair in two 16-bit halves.
 // Scales and zeros are [K / G][N rounded up to 16].
+//
+// A code becomes an operand with one AND-OR: c | 0x4300 is 128 + c in bf16, c | 0x6400 is 1024 + c in fp16, both exact.
+// The offset leaves again after each group of G features,
+//     sum x (c - z) = sum x (off + c) - (off + z) sum x,
+// where sum x comes from one more matrix instruction (its other operand is all ones), so scale and zero cost one fused
+// multiply-add per group and output, not one per weight.  All sums are fp32.
+//
+// The waves of a workgroup share R tiles of 16 outputs and split K between them, 128 features at a time; their sums meet in
+// LDS.  The next step's loads are in flight while a step is computed.
 #include "common.h"
 
 typedef _Float16 f16_t;
@@ -19,58 +28,314 @@ struct Int4Args {
   const void* res;
   void* y;
   long long x_rs, res_rs;
-  int M, N, K, G, act;
+  float* part;                                               // [kz][M][N rounded up to 16] sums of the parts of K
+  int M, N, K, act, kw, kz, z_on;                            // z_on: 1, or 0 where `zero` is one word of eights
 };
 
-// One wave per output column and four rows of x.
-template <typename T, typename S>
-__global__ __launch_bounds__(256) void int4_linear_kernel(const Int4Args a) {
-  const int lane = threadIdx.x & 63;
-  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), m0 = blockIdx.y * 4;
-  if (n >= a.N) return;
-  const int Ks = (a.K + 127) >> 7, Np = (a.N + 15) & ~15;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int e = lane; e < Ks * 16; e += 64) {
-    const int s = e >> 4, g = (e >> 2) & 3, i = e & 3;
-    const int k = s * 128 + i * 32 + g * 8;
-    if (k >= a.K) continue;
-    const uint32_t word = a.w[(((long long)(n >> 4) * Ks + s) * 64 + g * 16 + (n & 15)) * 4 + i];
-    const long long at = (long long)(k / a.G) * Np + n;
-    const float sc = (float)((const S*)a.scale)[at], z = a.zero ? (float)a.zero[at] : 8.f;
-    for (int m = 0; m < 4 && m0 + m < a.M; ++m) {
-      const T* xr = (const T*)a.x + (m0 + m) * a.x_rs + k;
-      float sum = 0.f;
+template <typename T> struct Mat4;
+template <> struct Mat4<bf16_t> {
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t BITS = 0x43004300u, ONE = 0x3f803f80u;
+  static constexpr float OFF = 128.f;
+  static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat4<f16_t> {
+  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t BITS = 0x64006400u, ONE = 0x3c003c00u;
+  static constexpr float OFF = 1024.f;
+  static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// What a wave holds of one step: 128 features of R tiles of 16 outputs and CT tiles of 16 rows.
+template <int R, int CT, int G>
+struct Step {
+  u32x4 x[CT][4];
+  u32x2 s[R][128 / G];                                       // scales of the lane's four outputs
+  uint32_t z[R][128 / G];
+};
+
+template <int R>
+__device__ __forceinline__ void load_words(u32x4 (&w)[R], const Int4Args& a, int s, int tile0, int tiles, int Ks, int lane) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += (float)xr[j] * ((float)((word >> (4 * (j >> 1) + 16 * (j & 1))) & 15u) - z);
-      acc[m] += sum * sc;
+  for (int i = 0; i < R; ++i)
+    w[i] = __builtin_nontemporal_load(
+        reinterpret_cast<const u32x4*>(a.w + (((long long)min(tile0 + i, tiles - 1) * Ks + s) * 64 + lane) * 4));
+}
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+typedef const uint8_t __attribute__((address_space(1)))* global_u8;    // said to be global memory: a generic load would wait for LDS too
+typedef const uint32_t __attribute__((address_space(1)))* global_u32;
+
+// x rows of the workgroup through a bounds-checked buffer: a lane whose row is not there has an offset outside and gets
+// zeros without a memory access and without a branch (a branch around loads would make the compiler wait for all of them).
+template <int R, int CT, int G>
+__device__ __forceinline__ void load_rest(Step<R, CT, G>& t, const Int4Args& a, global_u8 zero, rsrc_t x, const uint32_t (&xo)[CT], int s, int tile0,
+                                          int tiles, int g) {
+  const int Np = tiles * 16;
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.x[c][i] = __builtin_amdgcn_raw_buffer_load_b128(x, xo[c] + 64 * i, s * 256, 0);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int q = 0; q < 128 / G; ++q) {
+      const long long at = (long long)(s * (128 / G) + q) * Np + min(tile0 + i, tiles - 1) * 16 + 4 * g;
+      t.s[i][q] = *reinterpret_cast<const u32x2*>((const char*)a.scale + at * 2);
+      t.z[i][q] = *(global_u32)(zero + at * a.z_on);
+    }
+}
+
+// The last step of a K that is no multiple of 128: features from K on are zeros in x.
+template <int R, int CT, int G>
+__device__ __forceinline__ void load_rest_tail(Step<R, CT, G>& t, const Int4Args& a, global_u8 zero, rsrc_t x, const uint32_t (&xo)[CT], int s,
+                                               int tile0, int tiles, int g) {
+  const int Np = tiles * 16, groups = a.K / G;
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t.x[c][i] = u32x4{0u, 0u, 0u, 0u};
+      if (s * 128 + 32 * i < a.K) t.x[c][i] = __builtin_amdgcn_raw_buffer_load_b128(x, xo[c] + 64 * i, s * 256, 0);
+    }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int q = 0; q < 128 / G; ++q) {
+      const long long at = (long long)min(s * (128 / G) + q, groups - 1) * Np + min(tile0 + i, tiles - 1) * 16 + 4 * g;
+      t.s[i][q] = *reinterpret_cast<const u32x2*>((const char*)a.scale + at * 2);
+      t.z[i][q] = *(global_u32)(zero + at * a.z_on);
+    }
+}
+
+template <typename T, typename S, int R, int CT, int G>
+__device__ __forceinline__ void use_step(f32x4 (&y)[R][CT], const u32x4 (&words)[R], const Step<R, CT, G>& t) {
+  typedef typename Mat4<T>::x8 x8;
+  constexpr uint32_t BITS = Mat4<T>::BITS, ONE = Mat4<T>::ONE;
+  uint32_t nib = 0x000f000fu;
+  asm("" : "+v"(nib));                                       // in a vector register: AND-OR takes one scalar operand only
+  const x8 ones = __builtin_bit_cast(x8, u32x4{ONE, ONE, ONE, ONE});
+#pragma unroll
+  for (int q = 0; q < 128 / G; ++q) {
+    f32x4 acc[R][CT], xs[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      xs[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < R; ++i) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int i4 = q * (G / 32); i4 < (q + 1) * (G / 32); ++i4) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) xs[c] = Mat4<T>::mul(ones, __builtin_bit_cast(x8, t.x[c][i4]), xs[c]);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const uint32_t w = words[i][i4];
+        const u32x4 v = {(w & nib) | BITS, ((w >> 4) & nib) | BITS, ((w >> 8) & nib) | BITS, ((w >> 12) & nib) | BITS};
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[i][c] = Mat4<T>::mul(__builtin_bit_cast(x8, v), __builtin_bit_cast(x8, t.x[c][i4]), acc[i][c]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t h = j & 1 ? t.s[i][q][j >> 1] >> 16 : t.s[i][q][j >> 1] & 0xffffu;
+        const float s = (float)__builtin_bit_cast(S, (uint16_t)h);
+        const float z = Mat4<T>::OFF + (float)((t.z[i][q] >> (8 * j)) & 0xffu);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) y[i][c][j] += s * (acc[i][c][j] - z * xs[c][j]);
+      }
+    __builtin_amdgcn_sched_barrier(0);                       // one group's accumulators at a time
+  }
+}
+
+// bias, residual, activation, rounding of four consecutive outputs
+template <typename T>
+__device__ __forceinline__ void finish4(const Int4Args& a, f32x4 v, int m, int n) {
+  T* dst = (T*)a.y + (long long)m * a.N + n;
+  const T* rs = (const T*)a.res + m * a.res_rs + n;
+  T o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (n + j < a.N) {
+      float f = v[j];
+      if (a.bias) f += a.bias[n + j];
+      if (a.res) f += (float)rs[j];
+      o[j] = (T)dlamd_act(f, a.act);
+    }
+  }
+  if ((a.N & 3) == 0) {
+    *reinterpret_cast<u32x2*>(dst) = *reinterpret_cast<u32x2*>(o);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < a.N) dst[j] = o[j];
+  }
+}
+
+__device__ const uint32_t k_eights = 0x08080808u;             // the zeros of a layer without zeros
+
+// nw x kw waves: wave w takes the tiles of its w / kw and the steps w % kw, + kw, ... of the workgroup's part of K.
+template <typename T, typename S, int R, int CT, int G>
+__global__ __launch_bounds__(512) void int4_linear_kernel(const Int4Args a) {
+  const global_u8 zero = a.z_on ? (global_u8)a.zero : (global_u8)&k_eights;
+  extern __shared__ f32x4 s_y[];                             // [kw][nw R CT][lane]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int tiles = (a.N + 15) >> 4, Ks = (a.K + 127) >> 7;
+  const int nw = wave / a.kw, kw = wave - nw * a.kw, NW = (blockDim.x >> 6) / a.kw;
+  const int wg0 = blockIdx.x * R * NW, tile0 = wg0 + nw * R, m0 = blockIdx.y * 16 * CT;
+  const int per = (Ks + a.kz - 1) / a.kz, s0 = blockIdx.z * per, s1 = min(Ks, s0 + per);
+  f32x4 y[R][CT];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) y[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (tile0 < tiles) {
+    const int rows = min(16 * CT, a.M - m0);
+    const rsrc_t x = __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)a.x + m0 * a.x_rs), 0, (int)((rows - 1) * a.x_rs + a.K) * 2, 0x00020000);
+    uint32_t xo[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) xo[c] = 16 * c + r < rows ? (uint32_t)((16 * c + r) * a.x_rs * 2 + 16 * g) : 0x80000000u;
+    u32x4 w0[R], w1[R];
+    Step<R, CT, G> t0, t1;
+    const int full = min(s1, a.K >> 7);                      // steps [s0, full) have all 128 features
+    int s = s0 + kw, left = s < full ? (full - 1 - s) / a.kw + 1 : 0;
+    if (left == 1) {
+      load_words<R>(w0, a, s, tile0, tiles, Ks, lane);
+      load_rest<R, CT, G>(t0, a, zero, x, xo, s, tile0, tiles, g);
+      __builtin_amdgcn_sched_barrier(0);
+      use_step<T, S>(y, w0, t0);
+    } else if (left > 1) {
+      // Two steps in registers: one computes, one is in flight.  No load here has a condition: where paths with and without
+      // a load meet, the compiler can only wait for everything.
+      load_words<R>(w0, a, s, tile0, tiles, Ks, lane);
+      load_rest<R, CT, G>(t0, a, zero, x, xo, s, tile0, tiles, g);
+      __builtin_amdgcn_sched_barrier(0);
+      load_words<R>(w1, a, s + a.kw, tile0, tiles, Ks, lane);
+      load_rest<R, CT, G>(t1, a, zero, x, xo, s + a.kw, tile0, tiles, g);
+      __builtin_amdgcn_sched_barrier(0);
+      for (; left > 3; left -= 2, s += 2 * a.kw) {
+        use_step<T, S>(y, w0, t0);
+        load_words<R>(w0, a, s + 2 * a.kw, tile0, tiles, Ks, lane);
+        load_rest<R, CT, G>(t0, a, zero, x, xo, s + 2 * a.kw, tile0, tiles, g);
+        __builtin_amdgcn_sched_barrier(0);
+        use_step<T, S>(y, w1, t1);
+        load_words<R>(w1, a, s + 3 * a.kw, tile0, tiles, Ks, lane);
+        load_rest<R, CT, G>(t1, a, zero, x, xo, s + 3 * a.kw, tile0, tiles, g);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      use_step<T, S>(y, w0, t0);
+      if (left == 3) {
+        load_words<R>(w0, a, s + 2 * a.kw, tile0, tiles, Ks, lane);
+        load_rest<R, CT, G>(t0, a, zero, x, xo, s + 2 * a.kw, tile0, tiles, g);
+        __builtin_amdgcn_sched_barrier(0);
+        use_step<T, S>(y, w1, t1);
+        use_step<T, S>(y, w0, t0);
+      } else {
+        use_step<T, S>(y, w1, t1);
+      }
+    }
+    const bool tail = full < s1 && kw == (full - s0) % a.kw;
+    if (tail) {
+      load_words<R>(w0, a, full, tile0, tiles, Ks, lane);
+      load_rest_tail<R, CT, G>(t0, a, zero, x, xo, full, tile0, tiles, g);
+      use_step<T, S>(y, w0, t0);
     }
   }
 #pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    float v = wave_reduce_sum(acc[m]);
-    if (lane == 0 && m0 + m < a.M) {
-      if (a.bias) v += a.bias[n];
-      if (a.res) v += (float)((const T*)a.res)[(m0 + m) * a.res_rs + n];
-      ((T*)a.y)[(long long)(m0 + m) * a.N + n] = (T)dlamd_act(v, a.act);
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) s_y[((kw * NW * R + nw * R + i) * CT + c) * 64 + lane] = y[i][c];
+  __syncthreads();
+  // an item: four consecutive outputs of one row; consecutive threads take consecutive outputs
+  const int RT = R * NW;
+  for (int e = threadIdx.x; e < RT * CT * 64; e += blockDim.x) {
+    const int q = e % (4 * RT), rest = e / (4 * RT), rr = rest & 15, c = rest >> 4;
+    const int i = q >> 2, l = (q & 3) * 16 + rr;
+    const int m = m0 + 16 * c + rr, n = (wg0 + i) * 16 + 4 * (q & 3);
+    if (m >= a.M || n >= a.N) continue;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < a.kw; ++w) {
+      const f32x4 t = s_y[((w * RT + i) * CT + c) * 64 + l];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += t[j];
     }
+    if (a.kz == 1) finish4<T>(a, v, m, n);
+    else *reinterpret_cast<f32x4*>(a.part + ((long long)blockIdx.z * a.M + m) * (tiles * 16) + n) = v;
+  }
+}
+
+// Sums the parts of K and finishes: a thread per four outputs.
+template <typename T>
+__global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
+  const int Np = (a.N + 15) & ~15, per = Np >> 2;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(e / per), n = (int)(e - (long long)m * per) * 4;
+  if (m >= a.M || n >= a.N) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int z = 0; z < a.kz; ++z) {
+    const f32x4 t = *reinterpret_cast<const f32x4*>(a.part + ((long long)z * a.M + m) * Np + n);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += t[j];
+  }
+  finish4<T>(a, v, m, n);
+}
+
+template <typename T, typename S, int R, int CT, int G>
+static void launch4(const Int4Args& a, int nw, hipStream_t stream) {
+  const int per = R * nw;
+  const dim3 grid(((a.N + 15) / 16 + per - 1) / per, (a.M + 16 * CT - 1) / (16 * CT), a.kz);
+  hipLaunchKernelGGL((int4_linear_kernel<T, S, R, CT, G>), grid, dim3(nw * a.kw * 64), nw * a.kw * R * CT * 1024, stream, a);
+  if (a.kz > 1) {
+    const long long items = (long long)a.M * ((a.N + 15) / 16 * 4);
+    hipLaunchKernelGGL(int4_join_kernel<T>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
+  }
+}
+template <typename T, typename S, int R, int CT>
+static void launch4_g(const Int4Args& a, int G, int nw, hipStream_t stream) {
+  constexpr int R32 = R * CT == 8 ? 2 : R;                   // the scales of groups of 32 and 8 tiles do not fit the registers
+  if (G == 32) launch4<T, S, R32, CT, 32>(a, nw, stream);
+  else if (G == 64) launch4<T, S, R, CT, 64>(a, nw, stream);
+  else launch4<T, S, R, CT, 128>(a, nw, stream);
+}
+template <typename T, typename S>
+static void launch4_r(const Int4Args& a, int R, int CT, int G, int nw, hipStream_t stream) {
+  if (CT == 1) {
+    if (R == 1) launch4_g<T, S, 1, 1>(a, G, nw, stream);
+    else if (R == 2) launch4_g<T, S, 2, 1>(a, G, nw, stream);
+    else launch4_g<T, S, 4, 1>(a, G, nw, stream);
+  } else {
+    if (R == 1) launch4_g<T, S, 1, 2>(a, G, nw, stream);
+    else if (R == 2) launch4_g<T, S, 2, 2>(a, G, nw, stream);
+    else launch4_g<T, S, 4, 2>(a, G, nw, stream);
   }
 }
 
 // x: [M, K] (row stride given), y: [M, N] contiguous.  dtype, sdtype: 0 bf16, 1 fp16.  K % G == 0, G 32, 64 or 128.
+// A wave holds `tiles` (1, 2, 4) tiles of 16 outputs, a workgroup nw x kw <= 8 waves, K is split into kz parts over workgroups
+// (part: [kz][M][N rounded up to 16] floats where kz > 1).
 extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, const void* scale, const void* zero,
                                  const void* bias, const void* res, long long res_rs, void* y, int M, int N, int K, int G,
-                                 int act, int dtype, int sdtype, hipStream_t stream) {
+                                 int act, int dtype, int sdtype, int tiles, int nw, int kw, int kz, void* part,
+                                 hipStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || (G != 32 && G != 64 && G != 128) || K % G != 0) return -1;
-  if (x_rs % 8 != 0 || (((uintptr_t)x | (uintptr_t)w) & 15)) return -2;
+  if (K <= 0 || (G != 32 && G != 64 && G != 128) || K % G != 0 || N > 0x7ffffff0) return -1;
+  if (x_rs < 0 || x_rs >= (1 << 24) || K >= (1 << 24)) return -9;   // a workgroup's 32 rows of x: 31-bit offsets
+  if (x_rs % 8 != 0 || (((uintptr_t)x | (uintptr_t)w) & 15) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3) || ((uintptr_t)y & 7)) return -2;
   if ((dtype != 0 && dtype != 1) || (sdtype != 0 && sdtype != 1)) return -3;
   if (act != ACT_NONE && act != ACT_RELU && act != ACT_GELU) return -4;
-  Int4Args a{x, (const uint32_t*)w, scale, (const uint8_t*)zero, (const float*)bias, res, y, x_rs, res_rs, M, N, K, G, act};
-  const dim3 grid((N + 3) / 4, (M + 3) / 4);
-  if (grid.y > 65535) return -5;
-  if (dtype == 0 && sdtype == 0) hipLaunchKernelGGL((int4_linear_kernel<bf16_t, bf16_t>), grid, dim3(256), 0, stream, a);
-  if (dtype == 0 && sdtype == 1) hipLaunchKernelGGL((int4_linear_kernel<bf16_t, f16_t>), grid, dim3(256), 0, stream, a);
-  if (dtype == 1 && sdtype == 0) hipLaunchKernelGGL((int4_linear_kernel<f16_t, bf16_t>), grid, dim3(256), 0, stream, a);
-  if (dtype == 1 && sdtype == 1) hipLaunchKernelGGL((int4_linear_kernel<f16_t, f16_t>), grid, dim3(256), 0, stream, a);
+  const int CT = M <= 16 ? 1 : 2;
+  if ((M + 16 * CT - 1) / (16 * CT) > 65535) return -5;
+  if ((tiles != 1 && tiles != 2 && tiles != 4) || nw < 1 || kw < 1 || nw * kw > 8 || nw * kw * tiles * CT > 64) return -6;
+  if (kz < 1 || kz > 64 || (kz > 1 && (!part || ((uintptr_t)part & 15)))) return -7;
+  if ((long long)M * ((N + 15) / 16 * 4) > 0x7fffffffLL * 256) return -8;
+  Int4Args a{x, (const uint32_t*)w, scale, (const uint8_t*)zero, (const float*)bias, res, y, x_rs, res_rs, (float*)part,
+             M, N, K, act, kw, kz, zero ? 1 : 0};
+  if (dtype == 0 && sdtype == 0) launch4_r<bf16_t, bf16_t>(a, tiles, CT, G, nw, stream);
+  if (dtype == 0 && sdtype == 1) launch4_r<bf16_t, f16_t>(a, tiles, CT, G, nw, stream);
+  if (dtype == 1 && sdtype == 0) launch4_r<f16_t, bf16_t>(a, tiles, CT, G, nw, stream);
+  if (dtype == 1 && sdtype == 1) launch4_r<f16_t, f16_t>(a, tiles, CT, G, nw, stream);
   return DLAMD_CHECK_LAUNCH();
 }

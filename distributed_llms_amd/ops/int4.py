@@ -104,6 +104,16 @@ def linear_int4_reference(x, w: Int4Weight, bias=None, act: str = "none", res=No
     return _act_ref(y, act)
 
 
+def _shape(M: int, N: int, K: int):
+    """(tiles of 16 outputs a wave holds, waves over outputs, waves over K, parts of K over workgroups)."""
+    steps = -(-K // 128)
+    if N < 8192:
+        return 1, 1, min(8, steps), 1
+    if M <= 16:
+        return 2, 1, min(4, steps), 1
+    return 4, 1, min(4, steps), 2 if N < 10000 and steps >= 64 else 1
+
+
 def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None, *, act: str = "none",
                 res: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = act(x @ W^T + bias (+ res)) in x's type.  x: [..., K] bf16 or fp16, bias: fp32 [N], res: [..., N] of x's type;
@@ -133,9 +143,12 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
                 r2 = r2.contiguous()
         M = x2.shape[0]
         y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+        tiles, nw, kw, kz = _shape(M, N, K)
+        part = torch.empty((kz, M, -(-N // 16) * 16), dtype=torch.float32, device=dev) if kz > 1 else None
         rc = _loader.lib().dlamd_int4_linear(
             x2.data_ptr(), x2.stride(0), w.words.data_ptr(), w.scale.data_ptr(), 0 if w.zero is None else w.zero.data_ptr(),
             0 if bias is None else bias.data_ptr(), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
-            y.data_ptr(), M, N, K, w.group, _ACTS[act], _DTYPES[x.dtype], _DTYPES[w.scale.dtype], _loader.raw_stream(dev))
+            y.data_ptr(), M, N, K, w.group, _ACTS[act], _DTYPES[x.dtype], _DTYPES[w.scale.dtype], tiles, nw, kw, kz,
+            0 if part is None else part.data_ptr(), _loader.raw_stream(dev))
     _loader.check(rc, "dlamd_int4_linear")
     return y
