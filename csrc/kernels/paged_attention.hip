@@ -17,24 +17,30 @@
 //     then holds dimension (D / 16) r + i in row r, which leaves a lane with D / 4 consecutive dimensions of one query.
 //   * P goes into the products as two 16-bit halves, hi + lo: one rounding to 16 bits would cost as much accuracy as the
 //     result's own rounding, and the second product hides behind the loads.
-//   * Long sequences are split into chunks; each writes its (m, l, o) in 32 bits and a second kernel joins them.  The chunk
-//     is fixed by the host from the longest length a sequence may have, so a short sequence has few chunks and the
-//     workgroups of the others end at once.
+//   * Long caches are cut into parts of as many tiles (of 128 or 64 keys) as give every compute unit its share.  The size of a
+//     part is computed on the device from the lengths of the whole batch, so neither one long sequence nor a batch of very
+//     different lengths leaves compute units idle, and a captured call adapts while lengths grow.  A part is written as
+//     (m, l, o) in 32 bits and a second kernel joins the parts.  Short caches (and many of them) take one workgroup each.
 #include "common.h"
 
 typedef _Float16 f16_t;
+
+// Page table and lengths: constant memory to the compiler (the kernel's stores do not change them), so entries at uniform
+// places come by scalar loads, which do not wait for the tiles in flight.
+typedef const int __attribute__((address_space(4)))* const_i32;
 
 struct PagedAttArgs {
   const void *q, *kp, *vp;
   void* o;
   float* lse;
-  float* part;                                               // [units][splits][rows][D + 2]: o, then m, l
+  float* part;                                               // [workgroups][rows][D + 4]: o, then m, l
   const int *table, *lens;
   long long q_bs, q_ns, q_hs;
   long long k_ps, v_ps, t_bs;                                // page strides of the cache in bytes; table rows in entries
   int k_ss, k_hs, v_ss, v_hs;                                // slot / head strides in bytes
   int B, n, Hq, Hkv, page, width, pages, causal;
-  int splits, chunk, groups;                                 // chunk: keys per split; groups: row groups per (b, kv head)
+  int groups, rows, share, least;                            // row groups per (b, kv head), rows per group; workgroups to deal
+                                                             // tiles out to (0: one for each problem), least tiles of a part
   uint32_t page_magic;                                       // ceil(2^32 / (page / 16))
   float scale2;                                              // scale * log2(e)
 };
@@ -52,59 +58,70 @@ template <> struct Mat<f16_t> {
   static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
+typedef const char __attribute__((address_space(1)))* global_p;         // global memory, said so: no generic loads
+typedef const u32x4 __attribute__((address_space(1)))* global_u32x4;
+typedef const u32x2 __attribute__((address_space(1)))* global_u32x2;
+
+// What stands in for the rows of a page that does not exist: a row of zeros, read 16 times.
+__device__ const u32x4 k_zero_row[16] = {};
+
 // Where the two halves (16 keys, one page each) of a tile of 32 keys lie.
 struct Place {
-  const char *k[2], *v[2];                                   // the half's first key / value row
-  int last[2];                                               // last readable row of the half
+  global_p k[2], v[2];                                       // the half's first key / value row
+  int ks[2], vs[2];                                          // bytes from row to row, 0 for the row of zeros
+  int last[2];                                               // last row of the half below the limit
   bool ok[2];                                                // the half's page exists and some row sees it
 };
 
 // Page of the 16 keys at `key` (beyond the limit: none).  Uniform over the wave: the entry comes by a scalar load.
-__device__ __forceinline__ int page_of(const PagedAttArgs& p, const int* row, int key, int limit) {
+__device__ __forceinline__ int page_of(const PagedAttArgs& p, const_i32 row, int key, int limit) {
   const int unit = key >> 4;
   const int pi = p.page_magic ? (int)__umulhi((uint32_t)unit, p.page_magic) : unit;
   return key < limit ? row[pi] : -1;
 }
 
-// Rows that no one sees are not skipped but replaced by rows that are there (the limit's last one, or page 0): loads then
-// have no branches, and what they bring is masked (keys) or cleared (values) afterwards.  kh, vh: the head's first byte.
-__device__ __forceinline__ void find_tile(Place& t, const PagedAttArgs& p, const char* kh, const char* vh, int pid0, int pid1,
-                                          int k0, int limit) {
+// Rows that no one sees are not skipped but replaced by rows that are there (the limit's last one, or zeros for a missing
+// page): loads then have no branches.  kh, vh: the head's first byte.
+__device__ __forceinline__ void find_tile(Place& t, const PagedAttArgs& p, global_p kh, global_p vh, int pid0, int pid1, int k0,
+                                          int limit) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int key = k0 + 16 * h, pid = h ? pid1 : pid0;
     const int unit = key >> 4;
     const int pi = p.page_magic ? (int)__umulhi((uint32_t)unit, p.page_magic) : unit;
+    const int slot = key - pi * p.page;
     t.ok[h] = pid >= 0 && pid < p.pages;
-    const int at = t.ok[h] ? pid : 0, slot = t.ok[h] ? key - pi * p.page : 0;
-    t.k[h] = kh + at * p.k_ps + slot * p.k_ss;
-    t.v[h] = vh + at * p.v_ps + slot * p.v_ss;
-    t.last[h] = t.ok[h] ? min(15, limit - 1 - key) : 15;
+    t.k[h] = t.ok[h] ? kh + pid * p.k_ps + slot * p.k_ss : (global_p)k_zero_row;
+    t.v[h] = t.ok[h] ? vh + pid * p.v_ps + slot * p.v_ss : (global_p)k_zero_row;
+    t.ks[h] = t.ok[h] ? p.k_ss : 0;
+    t.vs[h] = t.ok[h] ? p.v_ss : 0;
+    t.last[h] = limit - 1 - key;
   }
 }
 
-template <int D>
-__device__ __forceinline__ void load_k(u32x4 (&k)[2][D / 32], const PagedAttArgs& p, const Place& t, int r, int g) {
+// TAIL: the tile may reach beyond the limit.
+template <int D, bool TAIL>
+__device__ __forceinline__ void load_k(u32x4 (&k)[2][D / 32], const Place& t, int r, int g) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t off = __umul24(min(r, t.last[h]), p.k_ss) + 16 * g;
+    const uint32_t off = __umul24(TAIL && t.ok[h] ? min(r, t.last[h]) : r, t.ks[h]) + 16 * g;
 #pragma unroll
-    for (int s = 0; s < D / 32; ++s) k[h][s] = *reinterpret_cast<const u32x4*>(t.k[h] + off + 64 * s);
+    for (int s = 0; s < D / 32; ++s) k[h][s] = *(global_u32x4)(t.k[h] + off + 64 * s);
   }
 }
 
-template <int D>
-__device__ __forceinline__ void load_v(uint32_t (&v)[8][D / 32], const PagedAttArgs& p, const Place& t, int r, int g) {
+template <int D, bool TAIL>
+__device__ __forceinline__ void load_v(uint32_t (&v)[8][D / 32], const Place& t, int r, int g) {
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
-    const uint32_t off = __umul24(min(4 * g + (s & 3), t.last[s >> 2]), p.v_ss) + D / 8 * r;
-    const char* b = t.v[s >> 2];
+    const int row = 4 * g + (s & 3), h = s >> 2;
+    const uint32_t off = __umul24(TAIL && t.ok[h] ? min(row, t.last[h]) : row, t.vs[h]) + D / 8 * r;
     if (D == 128) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(b + off);
+      const u32x4 x = *(global_u32x4)(t.v[h] + off);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[s][i] = x[i];
     } else {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(b + off);
+      const u32x2 x = *(global_u32x2)(t.v[h] + off);
       v[s][0] = x[0];
       v[s][1] = x[1];
     }
@@ -120,7 +137,7 @@ struct Rows {                                                // what a wave hold
 };
 
 // Scores of one tile (in units of log 2), -inf where a row does not see the key.
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, bool TAIL>
 __device__ __forceinline__ void scores(f32x4 (&x)[MT][2], const Rows<T, D, MT>& w, const u32x4 (&k)[2][D / 32], const Place& t,
                                        const PagedAttArgs& p, int k0, int g) {
   typedef typename Mat<T>::x8 x8;
@@ -128,12 +145,12 @@ __device__ __forceinline__ void scores(f32x4 (&x)[MT][2], const Rows<T, D, MT>& 
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int seen = (t.ok[h] ? w.lim[mt] : 0) - (k0 + 16 * h + 4 * g);
+      const int seen = (t.ok[h] ? TAIL ? w.lim[mt] : 0x7fffffff : 0) - (k0 + 16 * h + 4 * g);
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) s = Mat<T>::mul(__builtin_bit_cast(x8, k[h][c]), w.q[mt][c], s);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[mt][h][j] = j < seen ? s[j] * p.scale2 : -INFINITY;
+      for (int j = 0; j < 4; ++j) x[mt][h][j] = (TAIL ? j < seen : t.ok[h]) ? s[j] * p.scale2 : -INFINITY;
     }
 }
 
@@ -174,19 +191,19 @@ __device__ __forceinline__ void weights(typename Mat<T>::x8 (&hi)[MT], typename 
 }
 
 // Weights times values into the rows' sums.
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, bool TAIL>
 __device__ __forceinline__ void add_values(Rows<T, D, MT>& w, uint32_t (&v)[8][D / 32], const typename Mat<T>::x8 (&hi)[MT],
-                                           const typename Mat<T>::x8 (&lo)[MT], const Place& t, bool all, int k0,
+                                           const typename Mat<T>::x8 (&lo)[MT], const Place& t, int k0,
                                            int limit_all, int limit, int g, bool& odd) {
   typedef typename Mat<T>::x8 x8;
-  if (!all) {
+  if (TAIL) {
     // Rows of later tokens see keys that rows of earlier ones do not.  A product of a hidden key's weight, 0, and a value
-    // that is no finite number would be NaN, so such values leave the product here and are added row by row at the end.
+    // that is no finite number would be NaN, so such values leave the product here, and the sums are taken once more at the end.
     constexpr uint32_t EXP = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       const int key = k0 + 16 * (s >> 2) + 4 * g + (s & 3);
-      const bool none = !t.ok[s >> 2] || key >= limit, some = key >= limit_all;
+      const bool none = key >= limit, some = key >= limit_all;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         if (none) v[s][c] = 0u;
@@ -212,63 +229,133 @@ __device__ __forceinline__ void add_values(Rows<T, D, MT>& w, uint32_t (&v)[8][D
   }
 }
 
-// What add_values left out: values that are no finite numbers, at the (less than n) positions that some rows see and others
-// do not.  Never in sane use: the weight is computed again, element by element.
-template <typename T, int D, int MT>
-__device__ __forceinline__ void add_odd_values(Rows<T, D, MT>& w, const PagedAttArgs& p, const int* row, int b, int hk, int row0,
-                                               int R, int G, int kb, int wave, int limit_all, int limit, int r, int g) {
-  constexpr uint32_t EXP = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+// The wave's sums of values once more, element by element, for data the products above do not serve: a value that is no
+// finite number at a position that some rows see and others do not (0 x NaN), or an infinite one (hi and lo weights of both
+// signs).  m and l stand.
+template <typename T, int D, int MT, int TK>
+__device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedAttArgs& p, const_i32 row, int b, int hk, int row0,
+                                                 int R, int G, int first, int limit, int r, int g) {
+  typedef typename Mat<T>::x8 x8;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) w.o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-  for (int key = max(kb, limit_all); key < limit; ++key) {
-    if ((((key - kb) >> 5) & 3) != wave) continue;
-    const int pi = key / p.page, pid = row[pi];
-    if (pid < 0 || pid >= p.pages) continue;
-    const long long slot = key - pi * p.page;
-    const T* kr = (const T*)((const char*)p.kp + pid * p.k_ps + slot * p.k_ss + (long long)hk * p.k_hs);
-    const T* vr = (const T*)((const char*)p.vp + pid * p.v_ps + slot * p.v_ss + (long long)hk * p.v_hs) + D / 4 * g;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int at = row0 + 16 * mt + r, i = at / G, h = hk * G + at - i * G;
-      if (at >= R || key >= w.lim[mt]) continue;
-      const T* qr = (const T*)p.q + b * p.q_bs + i * p.q_ns + h * p.q_hs;
-      float x = 0.f;
+  for (int k0 = first; k0 < limit; k0 += TK) {
 #pragma unroll 1
-      for (int d = 0; d < D; ++d) x += (float)qr[d] * (float)kr[d];
-      const float e = __builtin_amdgcn_exp2f(x * p.scale2 - w.m[mt]);
+    for (int key = k0; key < min(k0 + 32, limit); ++key) {
+      const int pi = key / p.page, pid = row[pi];
+      if (pid < 0 || pid >= p.pages) continue;
+      const long long slot = key - pi * p.page;
+      const T* kr = (const T*)((const char*)p.kp + pid * p.k_ps + slot * p.k_ss + (long long)hk * p.k_hs);
+      const T* vr = (const T*)((const char*)p.vp + pid * p.v_ps + slot * p.v_ss + (long long)hk * p.v_hs) + D / 4 * g;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int mt = 0; mt < MT; ++mt) {
+        const int at = row0 + 16 * mt + r, i = at / G, h = hk * G + at - i * G;
+        if (at >= R || key >= w.lim[mt]) continue;
+        const T* qr = (const T*)p.q + b * p.q_bs + i * p.q_ns + h * p.q_hs;
+        float x = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 8) {
+          const x8 a = *reinterpret_cast<const x8*>(qr + d), c = *reinterpret_cast<const x8*>(kr + d);
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {                   // the lane's sums: dimensions D / 4 g .. of its query
-          const uint32_t bits = *reinterpret_cast<const uint16_t*>(vr + D / 16 * j + c);
-          if ((bits & EXP) == EXP) w.o[mt][c][j] += e * (float)vr[D / 16 * j + c];
+          for (int j = 0; j < 8; ++j) x += (float)a[j] * (float)c[j];
         }
+        const float e = __builtin_amdgcn_exp2f(x * p.scale2 - w.m[mt]);
+#pragma unroll
+        for (int d = 0; d < D / 4; d += 8) {                 // the lane's sums: dimensions D / 4 g .. of its query
+          const x8 v = *reinterpret_cast<const x8*>(vr + d);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w.o[mt][(d + j) % (D / 16)][(d + j) / (D / 16)] += e * (float)v[j];
+        }
+      }
     }
   }
 }
 
-template <typename T, int D, int MT>
-__global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_attention_kernel(const PagedAttArgs p) {
+// Tiles of sequence b (at least one: an empty sequence's rows are written, too).
+template <int TK>
+__device__ __forceinline__ int tiles_of(const PagedAttArgs& p, int b) {
+  const int kept = ((const_i32)p.lens)[b], cap = p.width * p.page;
+  const int limit = kept < 0 || p.pages == 0 ? 0 : min(min(kept, cap) + (p.causal ? p.n : 0), cap);
+  return max(1, (limit + TK - 1) / TK);
+}
+
+// Sum over the lanes up to and with this one: shifts inside rows of 16 lanes, then the last lanes of rows to the rows behind.
+__device__ __forceinline__ int wave_scan_i32(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// How tiles are dealt out.  A problem is a sequence's key head and group of rows, H of them per sequence.  Parts have
+// max(least, all tiles / share) tiles, a problem's last one less, so there are at most share + problems of them; they are
+// numbered problem after problem.
+template <int TK>
+__device__ __forceinline__ int tiles_each(const PagedAttArgs& p, int H, int lane, int mine) {
+  int sum = mine;                                            // tiles of sequence `lane`
+  for (int b = lane + 64; b < p.B; b += 64) sum += tiles_of<TK>(p, b);
+  const int total = __builtin_amdgcn_readlane(wave_scan_i32(sum), 63) * H;
+  return max(p.least, (total + p.share - 1) / p.share);
+}
+
+template <typename T, int D, int MT, int RW>
+__global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(const PagedAttArgs p) {
   typedef typename Mat<T>::x8 x8;
+  constexpr int KW = 4 / RW, TK = 32 * KW;                   // RW waves over rows, KW over keys
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ float s_o[4][16][D + 4];                        // + 4: lanes of one group write 16 rows at once
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  int u = blockIdx.x;
-  const int split = u % p.splits;
-  u /= p.splits;
-  const int group = u % p.groups, bh = u / p.groups;
-  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  const int G = p.Hq / p.Hkv, R = p.n * G, row0 = group * 16 * MT;
-  const int kept = p.lens[b];
-  const int cap = p.width * p.page;
-  const int base = kept < 0 ? 0 : min(kept, cap), more = kept >= 0 && p.causal;
-  // limits of the group's first and last row; a chunk ends the last split only with the sequence
+  const int r = lane & 15, g = lane >> 4, rw = RW == 1 ? 0 : wave / KW, kw = RW == 1 ? wave : wave % KW;
+  const int G = p.Hq / p.Hkv, R = p.n * G, H = p.Hkv * p.groups;
+  const int cap = p.width * p.page, me = blockIdx.x;
+
+  // which problem and which of its tiles
+  int b, head, tile = 0, tiles = 0x7fffffff;
+  bool whole = true;
+  if (p.share == 0) {
+    b = me / H;
+    head = me - b * H;
+  } else {
+    const int t0 = lane < p.B ? tiles_of<TK>(p, lane) : 0;
+    const int each = tiles_each<TK>(p, H, lane, t0);
+    int begin = 0, src = -1, upto = 0, parts = 0;
+    b = 0;
+    for (; b < p.B; b += 64) {                               // the sequence of part `me`, 64 of them at a time
+      const int t = b == 0 ? t0 : b + lane < p.B ? tiles_of<TK>(p, b + lane) : 0;
+      parts = (t + each - 1) / each;
+      upto = begin + wave_scan_i32(parts * H);
+      const unsigned long long past = __ballot(upto > me);
+      if (past) {
+        src = __ffsll(past) - 1;
+        break;
+      }
+      begin = __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (src < 0) return;                                     // fewer parts than workgroups
+    b += src;
+    parts = __builtin_amdgcn_readlane(parts, src);
+    const int in = me - (__builtin_amdgcn_readlane(upto, src) - parts * H);
+    head = in / parts;
+    tile = (in - head * parts) * each;
+    tiles = each;
+    whole = parts == 1;
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  head = __builtin_amdgcn_readfirstlane(head);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+
+  const int hk = head / p.groups, row0 = (head - hk * p.groups) * p.rows + rw * 16 * MT;
+  const int kept = ((const_i32)p.lens)[b];
+  const int base = kept < 0 || p.pages == 0 ? 0 : min(kept, cap), more = kept >= 0 && p.pages > 0 && p.causal;
+  // limits of the wave's first and last row
   const int rl = min(row0 + 16 * MT, R) - 1;
   const int limit_all = min(base + (more ? row0 / G + 1 : 0), cap);
-  int limit = p.pages > 0 ? min(base + (more ? rl / G + 1 : 0), cap) : 0;
-  const int kb = split * p.chunk;
-  if (split > 0 && kb >= limit) return;                      // the join knows which chunks exist
-  if (split < p.splits - 1) limit = min(limit, kb + p.chunk);
+  const int limit = row0 < R ? (int)min((long long)min(base + (more ? rl / G + 1 : 0), cap), ((long long)tile + tiles) * TK) : 0;
 
   Rows<T, D, MT> w;
 #pragma unroll
@@ -289,41 +376,49 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
   }
   // The next tile's keys are fetched into the registers of this one's as soon as the scores have been taken, its values
   // after the products: at any time a wave has most of a tile in flight, and three waves fit a SIMD.
-  const int* row = p.table + b * p.t_bs;
-  const char *kh = (const char*)p.kp + (long long)hk * p.k_hs, *vh = (const char*)p.vp + (long long)hk * p.v_hs;
-  int k0 = kb + 32 * wave;
+  const const_i32 row = (const_i32)p.table + b * p.t_bs;
+  const global_p kh = (global_p)p.kp + (long long)hk * p.k_hs, vh = (global_p)p.vp + (long long)hk * p.v_hs;
+  const int kb = tile * TK;
+  int k0 = kb + 32 * kw;
   bool odd = false;
   if (k0 < limit) {
     u32x4 k[2][D / 32];
     uint32_t v[8][D / 32];
-    Place at;
-    find_tile(at, p, kh, vh, page_of(p, row, k0, limit), page_of(p, row, k0 + 16, limit), k0, limit);
-    load_k<D>(k, p, at, r, g);
-    load_v<D>(v, p, at, r, g);
-    int pid0 = page_of(p, row, k0 + 128, limit), pid1 = page_of(p, row, k0 + 144, limit);
-    while (true) {
-      const bool all = k0 + 32 <= limit_all && k0 + 32 <= limit && at.ok[0] && at.ok[1];
-      const int k1 = k0 + 128;
-      f32x4 x[MT][2];
-      scores<T, D, MT>(x, w, k, at, p, k0, g);
+    Place pl;
+    x8 hi[MT], lo[MT];
+    f32x4 x[MT][2];
+    find_tile(pl, p, kh, vh, page_of(p, row, k0, limit), page_of(p, row, k0 + 16, limit), k0, limit);
+    load_k<D, true>(k, pl, r, g);
+    load_v<D, true>(v, pl, r, g);
+    int pid0 = page_of(p, row, k0 + TK, limit), pid1 = page_of(p, row, k0 + TK + 16, limit);
+    // All tiles but a wave's last end more than 32 keys before the wave's limit, and its first row's limit is at most 31
+    // keys before that: every row sees them.  No load here has a condition: where a path with loads meets one without, the
+    // compiler can only wait for all of them.
+    for (; k0 + TK < limit; k0 += TK) {
+      scores<T, D, MT, false>(x, w, k, pl, p, k0, g);
       Place next;
-      if (k1 < limit) {
-        find_tile(next, p, kh, vh, pid0, pid1, k1, limit);
-        load_k<D>(k, p, next, r, g);
-        pid0 = page_of(p, row, k1 + 128, limit);
-        pid1 = page_of(p, row, k1 + 144, limit);
-      }
-      x8 hi[MT], lo[MT];
+      find_tile(next, p, kh, vh, pid0, pid1, k0 + TK, limit);
+      load_k<D, true>(k, next, r, g);
+      pid0 = page_of(p, row, k0 + 2 * TK, limit);
+      pid1 = page_of(p, row, k0 + 2 * TK + 16, limit);
       weights<T, D, MT>(hi, lo, w, x);
-      add_values<T, D, MT>(w, v, hi, lo, at, all, k0, limit_all, limit, g, odd);
-      if (k1 >= limit) break;
-      load_v<D>(v, p, next, r, g);
-      at = next;
-      k0 = k1;
+      add_values<T, D, MT, false>(w, v, hi, lo, pl, k0, limit_all, limit, g, odd);
+      load_v<D, true>(v, next, r, g);
+      pl = next;
     }
+    scores<T, D, MT, true>(x, w, k, pl, p, k0, g);
+    weights<T, D, MT>(hi, lo, w, x);
+    add_values<T, D, MT, true>(w, v, hi, lo, pl, k0, limit_all, limit, g, odd);
   }
-  if (__any(odd)) add_odd_values<T, D, MT>(w, p, row, b, hk, row0, R, G, kb, wave, limit_all, limit, r, g);
-  // join the four waves, 16 rows at a time
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd |= w.o[mt][i][j] != w.o[mt][i][j];
+  if (__any(odd)) add_values_again<T, D, MT, TK>(w, p, row, b, hk, row0, R, G, kb + 32 * kw, limit, r, g);
+  float* part = p.part + (long long)me * p.rows * (D + 4);
+  // join the waves over keys, 16 rows of each wave over rows at a time
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float l = w.l[mt];
@@ -342,36 +437,41 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
         *reinterpret_cast<f32x4*>(&s_o[wave][r][(D / 16) * (4 * g + j) + i]) = t;
       }
     __syncthreads();
-    // thread: row threadIdx / 16, D / 16 dimensions
-    const int row_ = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16), row = row0 + 16 * mt + row_;
-    if (row < R) {
-      const float m = fmaxf(fmaxf(s_m[0][row_], s_m[1][row_]), fmaxf(s_m[2][row_], s_m[3][row_]));
-      float f[4], sum = 0.f;
+    // a thread: D / 16 dimensions of a row
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        f[x] = __builtin_amdgcn_exp2f(s_m[x][row_] - m);
-        sum += f[x] * s_l[x][row_];
+    for (int q = 0; q < RW; ++q) {
+      const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
+      const int in = (q * MT + mt) * 16 + rr, row = (head - hk * p.groups) * p.rows + in;
+      if (in >= p.rows || row >= R) continue;
+      float m = s_m[q * KW][rr];
+#pragma unroll
+      for (int x = 1; x < KW; ++x) m = fmaxf(m, s_m[q * KW + x][rr]);
+      float f[KW], sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < KW; ++x) {
+        f[x] = __builtin_amdgcn_exp2f(s_m[q * KW + x][rr] - m);
+        sum += f[x] * s_l[q * KW + x][rr];
       }
       float o[D / 16];
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         o[d] = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[d] += f[x] * s_o[x][row_][d0 + d];
+        for (int x = 0; x < KW; ++x) o[d] += f[x] * s_o[q * KW + x][rr][d0 + d];
       }
-      const int i = row / G, h = hk * G + row - i * G;
-      const long long at = ((long long)b * p.n + i) * p.Hq + h;
-      if (p.splits == 1) {
+      if (whole) {
+        const int i = row / G, h = hk * G + row - i * G;
+        const long long to = ((long long)b * p.n + i) * p.Hq + h;
         const float inv = 1.f / sum;
         T t[D / 16];
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) t[d] = (T)(sum == 0.f ? 0.f : o[d] * inv);   // sum is NaN where a score is
-        T* dst = (T*)p.o + at * D + d0;
+        T* dst = (T*)p.o + to * D + d0;
 #pragma unroll
         for (int d = 0; d < D / 16; d += 4) *reinterpret_cast<u32x2*>(dst + d) = *reinterpret_cast<u32x2*>(t + d);
-        if (p.lse && d0 == 0) p.lse[at] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * LN2;
+        if (p.lse && d0 == 0) p.lse[to] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * LN2;
       } else {
-        float* dst = p.part + ((long long)at * p.splits + split) * (D + 4);
+        float* dst = part + in * (D + 4);
 #pragma unroll
         for (int d = 0; d < D / 16; d += 4) *reinterpret_cast<f32x4*>(dst + d0 + d) = f32x4{o[d], o[d + 1], o[d + 2], o[d + 3]};
         if (d0 == 0) {
@@ -383,27 +483,31 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
   }
 }
 
-// One workgroup per row: joins the chunks of its sequence.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttArgs p, int rows_per_group) {
-  constexpr int TD = D / 4, SL = 256 / TD;                   // threads per chunk (4 dimensions each), chunks side by side
+// One workgroup per row: joins the parts of its sequence.
+template <typename T, int D, int TK>
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttArgs p) {
+  constexpr int TD = D / 4, SL = 256 / TD;                   // threads per part (4 dimensions each), parts side by side
   __shared__ float s_o[SL][D];
   __shared__ float s_l[SL], s_m[SL];
-  const long long at = blockIdx.x;
-  const int h = (int)(at % p.Hq), i = (int)((at / p.Hq) % p.n), b = (int)(at / ((long long)p.Hq * p.n));
-  const int G = p.Hq / p.Hkv;
-  const int kept = p.lens[b], cap = p.width * p.page;
-  const int base = kept < 0 ? 0 : min(kept, cap), more = kept >= 0 && p.causal;
-  // as many chunks as the row's group has: the limit of the group's last row
-  const int row = i * G + h % G, rl = min((row / rows_per_group + 1) * rows_per_group, p.n * G) - 1;
-  const int limit = p.pages > 0 ? min(base + (more ? rl / G + 1 : 0), cap) : 0;
-  const int have = max(1, min(p.splits, (limit + p.chunk - 1) / p.chunk));
+  const long long to = blockIdx.x;
+  const int h = (int)(to % p.Hq), i = (int)((to / p.Hq) % p.n), b = (int)(to / ((long long)p.Hq * p.n));
+  const int G = p.Hq / p.Hkv, H = p.Hkv * p.groups, hk = h / G;
+  const int row = i * G + h - hk * G, group = row / p.rows, in = row - group * p.rows;
+  const int lane = threadIdx.x & 63;
+  const int t0 = lane < p.B ? tiles_of<TK>(p, lane) : 0;
+  const int each = tiles_each<TK>(p, H, lane, t0);
+  const int parts = (tiles_of<TK>(p, b) + each - 1) / each;
+  if (parts == 1) return;                                    // written already
+  int before = 0;                                            // parts of the sequences before this one
+  for (int x = lane; x < b; x += 64) before += ((x == lane ? t0 : tiles_of<TK>(p, x)) + each - 1) / each;
+  const int lo = __builtin_amdgcn_readlane(wave_scan_i32(before), 63) * H + (hk * p.groups + group) * parts;
   const int d = (threadIdx.x % TD) * 4, sl = threadIdx.x / TD;
-  const float* src = p.part + at * p.splits * (D + 4);
+  const float* src = p.part + (long long)in * (D + 4);
   float m = ROW_NONE, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = sl; s < have; s += SL) {
-    const float* q = src + (long long)s * (D + 4);
+#pragma unroll 4
+  for (int s = lo + sl; s < lo + parts; s += SL) {
+    const float* q = src + (long long)s * p.rows * (D + 4);
     const float ms = q[D], ls = q[D + 1], mn = fmaxf(m, ms);
     const f32x4 os = *reinterpret_cast<const f32x4*>(q + d);
     const float a = __builtin_amdgcn_exp2f(m - mn), c = __builtin_amdgcn_exp2f(ms - mn);
@@ -419,39 +523,41 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
   }
   __syncthreads();
   if (threadIdx.x < D) {
-    float top = ROW_NONE, sum = 0.f, v = 0.f;
+    float top = ROW_NONE, sum2 = 0.f, v = 0.f;
 #pragma unroll
     for (int x = 0; x < SL; ++x) top = fmaxf(top, s_m[x]);
 #pragma unroll
     for (int x = 0; x < SL; ++x) {
       const float f = __builtin_amdgcn_exp2f(s_m[x] - top);
-      sum += f * s_l[x];
+      sum2 += f * s_l[x];
       v += f * s_o[x][threadIdx.x];
     }
-    ((T*)p.o)[at * D + threadIdx.x] = (T)(sum == 0.f ? 0.f : v / sum);
-    if (p.lse && threadIdx.x == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2;
+    ((T*)p.o)[to * D + threadIdx.x] = (T)(sum2 == 0.f ? 0.f : v / sum2);
+    if (p.lse && threadIdx.x == 0) p.lse[to] = sum2 == 0.f ? -INFINITY : (top + __log2f(sum2)) * LN2;
   }
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, int RW>
 static void launch(const PagedAttArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attention_kernel<T, D, MT>), dim3((unsigned)(a.B * a.Hkv * a.groups * a.splits)), dim3(256), 0, stream, a);
-  if (a.splits > 1)
-    hipLaunchKernelGGL((paged_attention_join_kernel<T, D>), dim3((unsigned)(a.B * a.n * a.Hq)), dim3(256), 0, stream, a, 16 * MT);
+  const unsigned grid = a.share + a.B * a.Hkv * a.groups;
+  hipLaunchKernelGGL((paged_attention_kernel<T, D, MT, RW>), dim3(grid), dim3(256), 0, stream, a);
+  if (a.share)
+    hipLaunchKernelGGL((paged_attention_join_kernel<T, D, 128 / RW>), dim3((unsigned)(a.B * a.n * a.Hq)), dim3(256), 0, stream, a);
 }
 template <typename T, int D>
-static void launch_rows(const PagedAttArgs& a, int mt, hipStream_t stream) {
-  if (mt == 1) launch<T, D, 1>(a, stream);
-  else if (mt == 2) launch<T, D, 2>(a, stream);
-  else launch<T, D, 4>(a, stream);
+static void launch_rows(const PagedAttArgs& a, int R, hipStream_t stream) {
+  if (R <= 16) launch<T, D, 1, 1>(a, stream);
+  else if (R <= 32) launch<T, D, 2, 1>(a, stream);
+  else launch<T, D, 2, 2>(a, stream);
 }
 
 // q: [B, n, Hq, D] (strides given), o: [B, n, Hq, D] contiguous, lse: [B, n, Hq] or null.  dtype: 0 bf16, 1 fp16.
-// splits chunks of `chunk` keys (the last one takes the rest); part: [B n Hq][splits][D + 4] floats where splits > 1.
+// share: 0 (a workgroup per sequence, key head and group of rows) or workgroups to deal all tiles out to, in parts of at least
+// `least` tiles; part: [share + problems][rows][D + 4] floats where share > 0, rows = min(n Hq / Hkv, 64).
 extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_ns, long long q_hs, const void* kp,
                                      long long kp_ps, long long kp_ss, long long kp_hs, const void* vp, long long vp_ps,
                                      long long vp_ss, long long vp_hs, const void* table, long long t_bs,
-                                     const void* lens, void* o, void* lse, void* part, int splits, int chunk, int B, int n,
+                                     const void* lens, void* o, void* lse, void* part, int share, int least, int B, int n,
                                      int Hq, int Hkv, int D, int page, int width, int pages, int causal, float scale,
                                      int dtype, hipStream_t stream) {
   if (B <= 0 || n <= 0 || Hq <= 0) return 0;
@@ -465,23 +571,22 @@ extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_
       sl[3] > 0x7fffffff || page * sl[0] > 0x7fffffff || page * sl[1] > 0x7fffffff)
     return -11;
   // positions are 32-bit; the page of a position is a multiplication, exact while units * (page / 16) < 2^32
-  if ((long long)width * page > 0x7fffff00LL || (long long)width * (page / 16) * (page / 16) >= (1LL << 32)) return -5;
+  if ((long long)width * page > 0x7ff00000LL || (long long)width * (page / 16) * (page / 16) >= (1LL << 32)) return -5;
   if (dtype != 0 && dtype != 1) return -6;
-  if (splits < 1 || chunk < 128 || chunk % 128 != 0 || (long long)(splits - 1) * chunk > 0x7fffff00LL) return -7;
-  if (splits > 1 && (!part || ((uintptr_t)part & 15))) return -8;
-  const int R = n * (Hq / Hkv);
+  if (share < 0 || share > (1 << 20) || (share > 0 && (least < 1 || !part || ((uintptr_t)part & 15)))) return -7;
   if ((long long)n * Hq > 0x7fffffffLL || (long long)B * n * Hq > 0x7fffffffLL) return -9;
-  const int mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  const int groups = (R + 16 * mt - 1) / (16 * mt);
-  if ((long long)B * Hkv * groups * splits > 0x7fffffffLL) return -10;
+  // rows of one problem: up to 16 (one tile of queries), 32 (two), 64 (two waves with two)
+  const int R = n * (Hq / Hkv), rows = R < 64 ? R : 64, groups = (R + 63) / 64;
+  // problems, parts and tiles are counted in 32 bits
+  if (((long long)B * Hkv * groups + share) * ((long long)width * page / 64 + 2) > 0x7fffffffLL) return -10;
   const uint32_t units = (uint32_t)(page / 16);
   const uint32_t magic = units == 1 ? 0u : (uint32_t)((0x100000000ULL + units - 1) / units);
   PagedAttArgs a{q, kp, vp, o, (float*)lse, (float*)part, (const int*)table, (const int*)lens, q_bs, q_ns, q_hs,
                  kp_ps * 2, vp_ps * 2, t_bs, (int)sl[0], (int)sl[2], (int)sl[1], (int)sl[3], B, n, Hq, Hkv, page, width, pages, causal,
-                 splits, chunk, groups, magic, scale * 1.4426950408889634f};
-  if (dtype == 0 && D == 64) launch_rows<bf16_t, 64>(a, mt, stream);
-  if (dtype == 0 && D == 128) launch_rows<bf16_t, 128>(a, mt, stream);
-  if (dtype == 1 && D == 64) launch_rows<f16_t, 64>(a, mt, stream);
-  if (dtype == 1 && D == 128) launch_rows<f16_t, 128>(a, mt, stream);
+                 groups, rows, share, least, magic, scale * 1.4426950408889634f};
+  if (dtype == 0 && D == 64) launch_rows<bf16_t, 64>(a, R, stream);
+  if (dtype == 0 && D == 128) launch_rows<bf16_t, 128>(a, R, stream);
+  if (dtype == 1 && D == 64) launch_rows<f16_t, 64>(a, R, stream);
+  if (dtype == 1 && D == 128) launch_rows<f16_t, 128>(a, R, stream);
   return DLAMD_CHECK_LAUNCH();
 }

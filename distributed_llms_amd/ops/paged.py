@@ -179,14 +179,17 @@ def paged_attention_reference(q, k_pages, v_pages, table, lens, scale: Optional[
     return o, lse
 
 
-def _split(units: int, bound: int) -> Tuple[int, int]:
-    """(chunks a sequence is split into, keys per chunk) for ``units`` independent (sequence, key head, row group) problems
-    of at most ``bound`` positions."""
-    if units >= 512 or bound <= 512:
-        return 1, 128
-    want = -(-1024 // units)
-    chunk = max(256, -(-(-(-bound // want)) // 128) * 128)
-    return -(-bound // chunk), chunk
+def _share(problems: int, rows: int, bound: int, D: int) -> Tuple[int, int]:
+    """How a call's work is dealt out: (0, 0), a workgroup per problem (sequence, key head, group of rows), or (workgroups to
+    deal all tiles of keys out to, least tiles of a part)."""
+    tile = 128 if rows <= 32 else 64
+    if bound <= tile or (problems >= 192 and bound <= 1024):
+        return 0, 0
+    return 256 * (_RESIDENT[D][0] if rows <= 16 else _RESIDENT[D][1]), max(1, 8 * rows // tile)
+
+
+# workgroups of the kernel that are resident on a compute unit (by its registers): rows <= 16, more
+_RESIDENT = {64: (4, 3), 128: (3, 2)}
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
@@ -223,12 +226,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         lse = torch.empty((B, n, hq), dtype=torch.float32, device=dev) if return_lse else None
         rows = n * (hq // hkv)
         bound = width * page if max_len is None else min(max_len, width * page)
-        splits, chunk = _split(B * hkv * -(-rows // 64), bound)
-        part = torch.empty((B * n * hq, splits, D + 4), dtype=torch.float32, device=dev) if splits > 1 else None
+        problems = B * hkv * -(-rows // 64)
+        share, least = _share(problems, rows, bound, D)
+        part = torch.empty((share + problems, min(rows, 64), D + 4), dtype=torch.float32, device=dev) if share else None
         rc = _loader.lib().dlamd_paged_attention(
             q.data_ptr(), *q.stride()[:3], k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
             table.data_ptr(), table.stride(0), lens.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            0 if part is None else part.data_ptr(), splits, chunk, B, n, hq, hkv, D, page,
+            0 if part is None else part.data_ptr(), share, least, B, n, hq, hkv, D, page,
             width, pages, 1 if causal else 0, scale, _DTYPES[q.dtype], _loader.raw_stream(dev))
     _loader.check(rc, "dlamd_paged_attention")
     return (o, lse) if return_lse else o

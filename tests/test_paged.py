@@ -230,6 +230,8 @@ ATT = [
     ([33, 0, 600], 9, 256, 7, 1, 64, "fp16", False, "heads"),
     ([9] * 70, 2, 16, 4, 2, 64, "bf16", True, "plain"),
     ([700], 40, 32, 5, 1, 64, "bf16", True, "plain"),
+    ([300, 2], 10, 16, 8, 1, 128, "bf16", True, "plain"),
+    ([(i * 61) % 400 - 1 for i in range(130)], 1, 16, 3, 1, 64, "fp16", True, "joint"),
 ]
 
 
@@ -350,14 +352,15 @@ def test_attention_kernel_keeps_odd_values_from_rows_that_do_not_see_them(dt):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("case", [4, 6, 7, 8])
-@pytest.mark.parametrize("splits,chunk", [(2, 128), (3, 384), (40, 128), (1, 128)])
-def test_attention_kernel_splits(case, splits, chunk, monkeypatch):
-    """Any split gives the result, also one whose last chunk takes more than its share."""
+@pytest.mark.parametrize("case", [2, 4, 6, 7, 8, 10, 11, 12, 13])
+@pytest.mark.parametrize("share,least", [(0, 0), (1, 1), (2, 1), (7, 3), (64, 1), (700, 1), (256, 100000)])
+def test_attention_kernel_shares(case, share, least, monkeypatch):
+    """Any way of dealing the work out gives the result: one workgroup for all of it, borders inside sequences, heads and
+    groups of rows, more workgroups than tiles."""
     kept, n, page, hq, hkv, D, dt, causal, layout = ATT[case]
     c = att_case(case, kept, n, page, hq, hkv, D, DTYPES[dt], causal, layout)
     d = {x: on_gpu_with_strides(y) if torch.is_tensor(y) else y for x, y in c.items()}
-    monkeypatch.setattr(P, "_split", lambda units, bound: (splits, chunk))
+    monkeypatch.setattr(P, "_share", lambda *_: (share, least))
     o, lse = P.paged_attention(**d, return_lse=True)
     check_attention(c, o.cpu(), lse.cpu())
 
