@@ -138,7 +138,7 @@ def _declare(l: ctypes.CDLL) -> None:
     sig("dlamd_paged_append", [vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, vp, vp, vp, vp]
         + [i] * 11 + [vp])
     sig("dlamd_paged_attention", [vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, vp, vp, vp, vp] + [i] * 11 + [f, i, vp])
-    sig("dlamd_verify_draft", [vp, ll, vp, ll, ll, vp, ll, ll, vp, ll, vp, vp, vp, i, i, i, i, i, vp])
+    sig("dlamd_verify_draft", [vp, ll, vp, ll, ll, vp, ll, ll, vp, ll, vp, vp, vp, vp] + [i] * 6 + [vp])
     sig("dlamd_int4_linear", [vp, ll, vp, vp, vp, vp, vp, ll, vp] + [i] * 11 + [vp, vp])
     sig("dlamd_embed_rows", [vp, vp, vp, vp, vp, ll, i, i, i, i, f, vp])
     sig("dlamd_decode_bookkeep", [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp])

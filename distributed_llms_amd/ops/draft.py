@@ -57,6 +57,13 @@ def verify_draft_reference(draft, target, u, proposal=None, counts=None, pad: in
     return tokens.to(draft.device), accepted.to(draft.device)
 
 
+def _pieces(B: int, V: int) -> int:
+    """Workgroups that share a row."""
+    if V <= 8192 or B >= 128:
+        return 1
+    return min(48, -(-V // 512)) if B < 32 else min(32, -(-V // 2048))
+
+
 def verify_draft(draft: torch.Tensor, target: torch.Tensor, u: torch.Tensor, proposal: Optional[torch.Tensor] = None,
                  counts: Optional[torch.Tensor] = None, pad: int = -1) -> Tuple[torch.Tensor, torch.Tensor]:
     """draft: int32 [B, n], the drafted tokens (0 <= n <= 63).  target: [B, n + 1, V] probabilities of the target model at
@@ -100,10 +107,12 @@ def verify_draft(draft: torch.Tensor, target: torch.Tensor, u: torch.Tensor, pro
         accepted = torch.empty((B,), dtype=torch.int32, device=dev)
         if n == 0:
             proposal = None
+        pieces = _pieces(B, V)
+        sums = torch.empty((B, pieces, 2), dtype=torch.float64, device=dev) if pieces > 1 else None
         rc = _loader.lib().dlamd_verify_draft(
             draft.data_ptr(), draft.stride(0), target.data_ptr(), target.stride(0), target.stride(1),
             0 if proposal is None else proposal.data_ptr(), 0 if proposal is None else proposal.stride(0),
             0 if proposal is None else proposal.stride(1), u.data_ptr(), u.stride(0), 0 if counts is None else counts.data_ptr(),
-            tokens.data_ptr(), accepted.data_ptr(), B, n, V, int(pad), _DTYPES[dt], _loader.raw_stream(dev))
+            tokens.data_ptr(), accepted.data_ptr(), 0 if sums is None else sums.data_ptr(), pieces, B, n, V, int(pad), _DTYPES[dt], _loader.raw_stream(dev))
     _loader.check(rc, "dlamd_verify_draft")
     return tokens, accepted

@@ -61,6 +61,8 @@ CASES = [  # B, n, V, dtype, proposal, ragged
     (7, 7, 272, "fp32", True, True), (5, 3, 1000, "fp16", False, True), (64, 5, 4097, "bf16", True, False),
     (2, 63, 97, "fp32", True, True), (2, 2, 151937, "fp32", False, False), (300, 1, 65, "fp32", True, True),
     (4, 3, 30011, "bf16", True, False), (40, 0, 777, "fp16", False, False),
+    (130, 2, 9001, "fp16", True, True), (3, 2, 8192, "fp32", True, True), (3, 2, 8193, "bf16", False, True), (5, 2, 1024, "fp32", True, True),
+    (2, 1, 1025, "fp32", True, True), (33, 2, 20011, "fp32", True, True),
 ]
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
