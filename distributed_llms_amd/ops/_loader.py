@@ -9,7 +9,6 @@ raises instead of silently falling back to eager PyTorch.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -58,18 +57,14 @@ def stream_ptr() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def raw_stream(device: torch.device) -> int:
-    """Handle of the current stream of a tensor's device."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+"""Handle of the current stream of a device, by its index."""
 
 
-_HERE = contextlib.nullcontext()
-
-
-def device_of(t: torch.Tensor):
-    """Context in which a tensor's device is the current one (kernels launch on the current device); costs nothing where
-    it already is."""
-    return _HERE if torch._C._cuda_getDevice() == t.device.index else torch.cuda.device(t.device)
+def elsewhere(index: int) -> bool:
+    """Whether device ``index`` is not the current one (kernels launch on the current device: the caller then enters
+    ``torch.cuda.device(index)`` first)."""
+    return torch._C._cuda_getDevice() != index
 
 
 def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:

@@ -96,23 +96,28 @@ def verify_draft(draft: torch.Tensor, target: torch.Tensor, u: torch.Tensor, pro
         raise ValueError("counts is int32 [B]")
     if target.stride(2) != 1 or draft.stride(1) != 1:
         raise ValueError("the last dimension of target and draft has to be contiguous")
-    dev = draft.device
-    for x in (target, u, proposal, counts):
-        if x is not None and x.device != dev:
-            raise ValueError("all tensors live on one device")
-    if not draft.is_cuda:
+    dev = draft.get_device()
+    if (target.get_device() != dev or u.get_device() != dev or (proposal is not None and proposal.get_device() != dev)
+            or (counts is not None and counts.get_device() != dev)):
+        raise ValueError("all tensors live on one device")
+    if dev < 0:
         return verify_draft_reference(draft, target, u, proposal, counts, pad)
-    with _loader.device_of(draft):
-        tokens = torch.empty((B, n + 1), dtype=torch.int32, device=dev)
-        accepted = torch.empty((B,), dtype=torch.int32, device=dev)
-        if n == 0:
-            proposal = None
-        pieces = _pieces(B, V)
-        sums = torch.empty((B, pieces, 2), dtype=torch.float64, device=dev) if pieces > 1 else None
-        rc = _loader.lib().dlamd_verify_draft(
-            draft.data_ptr(), draft.stride(0), target.data_ptr(), target.stride(0), target.stride(1),
-            0 if proposal is None else proposal.data_ptr(), 0 if proposal is None else proposal.stride(0),
-            0 if proposal is None else proposal.stride(1), u.data_ptr(), u.stride(0), 0 if counts is None else counts.data_ptr(),
-            tokens.data_ptr(), accepted.data_ptr(), 0 if sums is None else sums.data_ptr(), pieces, B, n, V, int(pad), _DTYPES[dt], _loader.raw_stream(dev))
-    _loader.check(rc, "dlamd_verify_draft")
+    if _loader.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return verify_draft(draft, target, u, proposal, counts, pad)
+    tokens = draft.new_empty((B, n + 1))
+    accepted = draft.new_empty((B,))
+    q_p = q_bs = q_ns = 0
+    if proposal is not None and n:
+        q_p = proposal.data_ptr()
+        q_bs, q_ns, _ = proposal.stride()
+    p_bs, p_ns, _ = target.stride()
+    pieces = _pieces(B, V)
+    sums = draft.new_empty((B, pieces, 2), dtype=torch.float64) if pieces > 1 else None
+    rc = _loader.lib().dlamd_verify_draft(
+        draft.data_ptr(), draft.stride(0), target.data_ptr(), p_bs, p_ns, q_p, q_bs, q_ns, u.data_ptr(), u.stride(0),
+        0 if counts is None else counts.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), 0 if sums is None else sums.data_ptr(),
+        pieces, B, n, V, pad, _DTYPES[dt], _loader.raw_stream(dev))
+    if rc:
+        _loader.check(rc, "dlamd_verify_draft")
     return tokens, accepted

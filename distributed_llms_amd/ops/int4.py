@@ -127,28 +127,34 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
         raise ValueError("bias is fp32 [N]")
     if res is not None and (res.shape[:-1] != x.shape[:-1] or res.shape[-1] != N or res.dtype != x.dtype):
         raise ValueError("res is [..., N] of x's type")
-    dev = x.device
-    if w.words.device != dev or (bias is not None and bias.device != dev) or (res is not None and res.device != dev):
+    dev = x.get_device()
+    if w.words.get_device() != dev or (bias is not None and bias.get_device() != dev) or (res is not None and res.get_device() != dev):
         raise ValueError("all tensors live on one device")
-    if not x.is_cuda:
+    if dev < 0:
         return linear_int4_reference(x, w, bias, act, res).to(x.dtype)
-    with _loader.device_of(x):
-        x2 = x if x.dim() == 2 else x.reshape(-1, K)
-        if x2.stride(1) != 1 or x2.stride(0) % 8 != 0 or x2.data_ptr() % 16 != 0:
-            x2 = x2.contiguous() if not x2.is_contiguous() else x2.clone()      # rows the kernel can load 16 bytes at a time
-        r2 = None
-        if res is not None:
-            r2 = res if res.dim() == 2 else res.reshape(-1, N)
-            if r2.stride(1) != 1:
-                r2 = r2.contiguous()
-        M = x2.shape[0]
-        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
-        tiles, nw, kw, kz = _shape(M, N, K)
-        part = torch.empty((kz, M, -(-N // 16) * 16), dtype=torch.float32, device=dev) if kz > 1 else None
-        rc = _loader.lib().dlamd_int4_linear(
-            x2.data_ptr(), x2.stride(0), w.words.data_ptr(), w.scale.data_ptr(), 0 if w.zero is None else w.zero.data_ptr(),
-            0 if bias is None else bias.data_ptr(), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
-            y.data_ptr(), M, N, K, w.group, _ACTS[act], _DTYPES[x.dtype], _DTYPES[w.scale.dtype], tiles, nw, kw, kz,
-            0 if part is None else part.data_ptr(), _loader.raw_stream(dev))
-    _loader.check(rc, "dlamd_int4_linear")
+    if _loader.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return linear_int4(x, w, bias, act=act, res=res)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    x_rs, x_ks = x2.stride()
+    if x_ks != 1 or x_rs % 8 != 0 or x2.data_ptr() % 16 != 0:
+        # rows the kernel cannot load 16 bytes at a time
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+        x_rs = K
+    M = x2.shape[0]
+    r2_p = r_rs = 0
+    if res is not None:
+        r2 = res if res.dim() == 2 else res.reshape(-1, N)
+        if r2.stride(1) != 1:
+            r2 = r2.contiguous()
+        r2_p, r_rs = r2.data_ptr(), r2.stride(0)
+    y = x.new_empty((*x.shape[:-1], N))
+    tiles, nw, kw, kz = _shape(M, N, K)
+    part = x.new_empty((kz, M, -(-N // 16) * 16), dtype=torch.float32) if kz > 1 else None
+    rc = _loader.lib().dlamd_int4_linear(
+        x2.data_ptr(), x_rs, w.words.data_ptr(), w.scale.data_ptr(), 0 if w.zero is None else w.zero.data_ptr(),
+        0 if bias is None else bias.data_ptr(), r2_p, r_rs, y.data_ptr(), M, N, K, w.group, _ACTS[act], _DTYPES[x.dtype],
+        _DTYPES[w.scale.dtype], tiles, nw, kw, kz, 0 if part is None else part.data_ptr(), _loader.raw_stream(dev))
+    if rc:
+        _loader.check(rc, "dlamd_int4_linear")
     return y
