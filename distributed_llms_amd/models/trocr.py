@@ -38,6 +38,8 @@ import torch.nn.functional as F
 from ..ops import ctc as ctc_ops
 from ..ops import transformer as T
 from ..ops.conv import conv2d_nhwc, linear_bf16
+from ..ops.int4 import Int4Weight, linear_int4, quantize_int4
+from ..ops.paged import paged_append, paged_attention
 
 
 @dataclass
@@ -121,6 +123,17 @@ def _pk(lin: nn.Linear):
     return lin.weight.detach().to(torch.bfloat16).contiguous(), lin.bias.detach().float().contiguous()
 
 
+def _pk4(lin: nn.Linear, group: int):
+    return quantize_int4(lin.weight, group), lin.bias.detach().float().contiguous()
+
+
+def _linear(x: torch.Tensor, w, bias, act: str = "none", res: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A decoder layer's linear on weights as ``prepare`` packed them: bf16 or 4-bit."""
+    if isinstance(w, Int4Weight):
+        return linear_int4(x, w, bias, act=act, res=res)
+    return linear_bf16(x, w, bias, act=act, res=res)
+
+
 def _ln(ln: nn.LayerNorm):
     return ln.weight.detach().float().contiguous(), ln.bias.detach().float().contiguous()
 
@@ -150,6 +163,7 @@ class TrOCR(nn.Module):
                 nn.init.normal_(m.weight, std=0.02)
         self._pk: Optional[Dict] = None
         self._graphs: Dict[int, "_DecodeGraph"] = {}
+        self.int4_group = 0
 
     def _apply(self, fn, *a, **k):
         self._pk = None
@@ -204,9 +218,17 @@ class TrOCR(nn.Module):
         return toks[:, 1:]
 
     # ------------------------------------------------------------------ MI355X inference path
-    def prepare(self) -> "TrOCR":
+    def prepare(self, int4_group: Optional[int] = None) -> "TrOCR":
+        """Pack the weights for inference.  ``int4_group`` (32, 64 or 128; None keeps the last choice, 0 = bf16): the
+        decoder's linears and the vocabulary projection as 4-bit weights with one scale per so many input features - a decode
+        step then reads a quarter of the weight bytes, which is what a small batch waits for; a batch of hundreds of crops is
+        served better by bf16.  The encoder and the cross-attention keys / values (hundreds of rows per crop) stay bf16."""
         self.eval()
         cfg = self.cfg
+        if int4_group is not None:
+            self.int4_group = int4_group
+        g4 = self.int4_group
+        dec = (lambda lin: _pk4(lin, g4)) if g4 else _pk
         dev = self.lm_head.weight.device
         pk: Dict = {}
         w = self.patch_embed.weight.detach().float()                       # [D, 3, p, p]
@@ -218,8 +240,8 @@ class TrOCR(nn.Module):
         pk["enc"] = [dict(ln1=_ln(l.ln1), ln2=_ln(l.ln2), qkv=_pk(l.qkv), proj=_pk(l.proj), fc1=_pk(l.fc1),
                           fc2=_pk(l.fc2)) for l in self.enc]
         pk["enc_ln"] = _ln(self.enc_ln)
-        pk["dec"] = [dict(ln1=_ln(l.ln1), ln2=_ln(l.ln2), ln3=_ln(l.ln3), qkv=_pk(l.qkv), proj=_pk(l.proj),
-                          xq=_pk(l.xq), xkv=_pk(l.xkv), xproj=_pk(l.xproj), fc1=_pk(l.fc1), fc2=_pk(l.fc2))
+        pk["dec"] = [dict(ln1=_ln(l.ln1), ln2=_ln(l.ln2), ln3=_ln(l.ln3), qkv=dec(l.qkv), proj=dec(l.proj),
+                          xq=dec(l.xq), xkv=_pk(l.xkv), xproj=dec(l.xproj), fc1=dec(l.fc1), fc2=dec(l.fc2))
                      for l in self.dec]
         pk["dec_ln"] = _ln(self.dec_ln) if self.dec_ln is not None else None
         pk["emb_ln"] = _ln(self.emb_ln) if self.emb_ln is not None else None
@@ -229,7 +251,7 @@ class TrOCR(nn.Module):
         lw[: cfg.vocab] = self.lm_head.weight.detach().float()
         lb = torch.full((cfg.vocab_padded,), -1e4, device=dev)
         lb[: cfg.vocab] = 0.0
-        pk["lm"] = (lw.to(torch.bfloat16).contiguous(), lb.contiguous())
+        pk["lm"] = (quantize_int4(lw, g4) if g4 else lw.to(torch.bfloat16).contiguous(), lb.contiguous())
         self._pk = pk
         self._graphs = {}
         return self
@@ -268,29 +290,28 @@ class TrOCR(nn.Module):
         post = cfg.post_ln
         for li, l in enumerate(pk["dec"]):
             y = x if post else T.layernorm(x, *l["ln1"])
-            qkv = linear_bf16(y, *l["qkv"])
-            a = T.attention_decode(qkv[:, :d], st.k_self[li], st.v_self[li], cfg.dec_heads,
-                                   k_new=qkv[:, d : 2 * d], v_new=qkv[:, 2 * d :], t=st.t)
-            x = linear_bf16(a, *l["proj"], res=x)
+            a = st.attend_self(li, _linear(y, *l["qkv"]))
+            x = _linear(a, *l["proj"], res=x)
             if post:
                 x = T.layernorm(x, *l["ln1"])
             y = x if post else T.layernorm(x, *l["ln2"])
-            q = linear_bf16(y, *l["xq"])
-            a = T.attention_decode(q, st.k_cross[li], st.v_cross[li], cfg.dec_heads, klen=cfg.tokens)
-            x = linear_bf16(a, *l["xproj"], res=x)
+            a = st.attend_memory(li, _linear(y, *l["xq"]))
+            x = _linear(a, *l["xproj"], res=x)
             if post:
                 x = T.layernorm(x, *l["ln2"])
             y = x if post else T.layernorm(x, *l["ln3"])
-            y = linear_bf16(y, *l["fc1"], act=cfg.act)
-            x = linear_bf16(y, *l["fc2"], res=x)
+            y = _linear(y, *l["fc1"], act=cfg.act)
+            x = _linear(y, *l["fc2"], res=x)
             if post:
                 x = T.layernorm(x, *l["ln3"])
         if pk["dec_ln"] is not None:
             x = T.layernorm(x, *pk["dec_ln"])
-        logits = linear_bf16(x, *pk["lm"])
+        logits = _linear(x, *pk["lm"])
         ctc_ops.row_argmax(logits, out=(st.tokens, st.probs))
         # history, probability sums, EOS marks, step counter and the all-done flag: one small kernel inside the step
         T.decode_bookkeep(st.tokens, st.probs, st.t, st.out, st.psum, st.cnt, st.done, st.flag, cfg.eos)
+        if st.lens is not None:
+            st.lens.add_(1)
 
     ENC_CHUNK = 256
 
@@ -320,8 +341,8 @@ class TrOCR(nn.Module):
             mem = self.encode(x[c0 : c0 + self.ENC_CHUNK])
             for li, l in enumerate(pk["dec"]):
                 kv = linear_bf16(mem, *l["xkv"])
-                st.k_cross[li][c0 : c0 + mem.shape[0]].copy_(kv[..., : cfg.dec_dim])
-                st.v_cross[li][c0 : c0 + mem.shape[0]].copy_(kv[..., cfg.dec_dim :])
+                st.k_cross[li][c0 : c0 + mem.shape[0], : cfg.tokens].copy_(kv[..., : cfg.dec_dim])
+                st.v_cross[li][c0 : c0 + mem.shape[0], : cfg.tokens].copy_(kv[..., cfg.dec_dim :])
         st.reset(B, cfg)
         events = []
         steps = 0
@@ -371,21 +392,61 @@ class _DecodeState:
         self.tokens = torch.zeros((Bb,), dtype=torch.int32, device=device)
         self.probs = torch.zeros((Bb,), dtype=torch.float32, device=device)
         self.t = torch.zeros((1,), dtype=torch.int32, device=device)
-        self.k_self = [z(Bb, cfg.max_len, cfg.dec_dim) for _ in range(cfg.dec_layers)]
-        self.v_self = [z(Bb, cfg.max_len, cfg.dec_dim) for _ in range(cfg.dec_layers)]
-        self.k_cross = [z(Bb, cfg.tokens, cfg.dec_dim) for _ in range(cfg.dec_layers)]
-        self.v_cross = [z(Bb, cfg.tokens, cfg.dec_dim) for _ in range(cfg.dec_layers)]
+        on_gpu = torch.device(device).type == "cuda"
+        self.heads, self.memory = cfg.dec_heads, cfg.tokens
+        # ``attention_decode`` holds the scores of at most MAX_DECODE_KEYS keys: longer outputs and larger images keep their keys
+        # and values in pages (self-attention: PAGE tokens each; encoder tokens: one page per sequence)
+        i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=device)  # noqa: E731
+        self.lens = self.table = self.mem_lens = self.mem_table = None
+        cap, mem = cfg.max_len, cfg.tokens
+        if on_gpu and cap > T.MAX_DECODE_KEYS:
+            cap = -(-cap // self.PAGE) * self.PAGE
+            self.lens = i32(Bb)
+            self.table = i32(Bb, cap // self.PAGE)
+        if on_gpu and mem > T.MAX_DECODE_KEYS:
+            mem = -(-mem // 16) * 16
+            self.mem_lens = i32(Bb).fill_(cfg.tokens)
+            self.mem_table = torch.arange(Bb, dtype=torch.int32, device=device)[:, None].contiguous()
+        self.k_self = [z(Bb, cap, cfg.dec_dim) for _ in range(cfg.dec_layers)]
+        self.v_self = [z(Bb, cap, cfg.dec_dim) for _ in range(cfg.dec_layers)]
+        self.k_cross = [z(Bb, mem, cfg.dec_dim) for _ in range(cfg.dec_layers)]
+        self.v_cross = [z(Bb, mem, cfg.dec_dim) for _ in range(cfg.dec_layers)]
         # bookkeeping of the greedy loop, updated by the last kernel of every step (ops.transformer.decode_bookkeep)
         self.out = torch.full((cfg.max_len, Bb), cfg.pad, dtype=torch.int32, device=device)
         self.psum = torch.zeros((Bb,), dtype=torch.float32, device=device)
         self.cnt = torch.zeros((Bb,), dtype=torch.float32, device=device)
         self.done = torch.zeros((Bb,), dtype=torch.uint8, device=device)
-        on_gpu = torch.device(device).type == "cuda"
         # "every sequence has emitted eos", written by the device, read by the host without a stream synchronisation
         self.flag = torch.zeros((1,), dtype=torch.int32, pin_memory=True) if on_gpu else torch.zeros((1,), dtype=torch.int32)
 
+    PAGE = 64
+
+    def attend_self(self, li: int, qkv: torch.Tensor) -> torch.Tensor:
+        """Self-attention of the step's token: its key and value join the cache, its query reads all of it."""
+        B, d, k, v = qkv.shape[0], qkv.shape[1] // 3, self.k_self[li], self.v_self[li]
+        if self.lens is None:
+            return T.attention_decode(qkv[:, :d], k, v, self.heads, k_new=qkv[:, d : 2 * d], v_new=qkv[:, 2 * d :], t=self.t)
+        q, kn, vn = qkv.view(B, 3, self.heads, T.HEAD_DIM).unbind(1)
+        k, v = (x.view(-1, self.PAGE, self.heads, T.HEAD_DIM) for x in (k, v))
+        paged_append(kn, vn, k, v, self.table, self.lens)
+        return paged_attention(q[:, None], k, v, self.table, self.lens).view(B, d)
+
+    def attend_memory(self, li: int, q: torch.Tensor) -> torch.Tensor:
+        """Cross-attention of the step's token over the encoder's tokens."""
+        k, v = self.k_cross[li], self.v_cross[li]
+        if self.mem_lens is None:
+            return T.attention_decode(q, k, v, self.heads, klen=self.memory)
+        k, v = (x.view(*x.shape[:2], self.heads, T.HEAD_DIM) for x in (k, v))
+        o = paged_attention(q.view(-1, 1, self.heads, T.HEAD_DIM), k, v, self.mem_table, self.mem_lens, causal=False)
+        return o.view(q.shape)
+
     def reset(self, B: int, cfg) -> None:
         """Start a new batch of ``B`` sequences (rows beyond B are padding of the batch bucket: done from the start)."""
+        if self.lens is not None:
+            pages = self.table.shape[1]
+            self.lens.zero_()
+            self.table.copy_(torch.arange(self.table.numel(), dtype=torch.int32, device=self.table.device).view(-1, pages))
+            self.table[B:] = -1                              # no pages: padding rows write nothing and see nothing
         self.tokens.fill_(cfg.bos)
         self.t.zero_()
         self.out.fill_(cfg.pad)

@@ -12,6 +12,7 @@ import torch.nn.functional as F
 from . import _loader
 
 HEAD_DIM = 64
+MAX_DECODE_KEYS = 1024      # attention_decode keeps a sequence's scores in LDS; longer caches: ops.paged
 
 
 def layernorm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5,
