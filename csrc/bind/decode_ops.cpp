@@ -1,0 +1,358 @@
+// The host side of the decode-step operators (ops/paged.py, ops/int4.py, ops/draft.py) on device tensors: argument checks,
+// outputs and workspaces from PyTorch's allocator, the launch.
+//
+// A decode step is made of calls whose kernels take 3 to 10 us, so the host has to issue one in less than that.  In Python a
+// call cost 8.7 us (3.4 us of it the launch itself, 2.8 us two allocations, the rest reading sizes, strides and addresses one by
+// one); here 5 us.  The kernels are the plain C entries of libdlamd_kernels.so, whose addresses Python hands over once (init).
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <cmath>
+#include <stdexcept>
+#include <string>
+
+namespace {
+
+typedef long long ll;
+
+struct Refused : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+struct Failed : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
+void need(bool ok, const char* why) {
+  if (!ok) throw Refused(why);
+}
+void launched(int rc, const char* name) {
+  if (rc != 0)
+    throw Failed(std::string(name) + " failed with code " + std::to_string(rc) + " (host-side shape contract or launch error)");
+}
+
+int (*k_append)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, void*, void*, ll, ll, ll, void*, ll, ll, ll, const void*, ll,
+                const void*, const void*, const void*, const void*, int, int, int, int, int, int, int, int, int, int, int, void*);
+int (*k_attention)(const void*, ll, ll, ll, const void*, ll, ll, ll, const void*, ll, ll, ll, const void*, ll, const void*, void*, void*, void*,
+                   int, int, int, int, int, int, int, int, int, int, int, float, int, void*);
+int (*k_verify)(const void*, ll, const void*, ll, ll, const void*, ll, ll, const void*, ll, const void*, void*, void*, void*, int, int, int, int,
+                int, int, void*);
+int (*k_int4)(const void*, ll, const void*, const void*, const void*, const void*, const void*, ll, void*, int, int, int, int, int, int, int, int,
+              int, int, int, void*, void*);
+PyObject* k_error = nullptr;                                 // the framework's KernelLibraryError
+
+// ------------------------------------------------------------------------------------------ arguments
+struct Maybe {
+  const at::Tensor* t = nullptr;
+  explicit operator bool() const { return t != nullptr; }
+  const at::Tensor* operator->() const { return t; }
+  const void* ptr() const { return t ? t->data_ptr() : nullptr; }
+};
+Maybe maybe(PyObject* o) {
+  if (o == Py_None) return {};
+  need(THPVariable_Check(o), "a tensor or None is expected");
+  return {&THPVariable_Unpack(o)};
+}
+const at::Tensor& tensor(PyObject* o) {
+  need(THPVariable_Check(o), "a tensor is expected");
+  return THPVariable_Unpack(o);
+}
+ll number(PyObject* o) {
+  const ll v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    throw Refused("a whole number is expected");
+  }
+  return v;
+}
+bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+
+// Device of the call, made current for the launch, and its current stream as Python knows it.
+struct Where {
+  c10::DeviceGuard guard;
+  void* stream;
+  Where(const at::Tensor& t, PyObject* s) : guard(t.device()), stream((void*)(intptr_t)number(s)) {}
+};
+void same_device(const c10::Device& d, std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts) need(!t || t->device() == d, "all tensors live on one device");
+}
+
+int half_type(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : -1; }
+
+void check_cache(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& table, const at::Tensor& lens) {
+  need(kp.dim() == 4 && vp.sizes() == kp.sizes(), "k_pages and v_pages are [pages, page, kv_heads, D] of one shape");
+  need(half_type(kp.scalar_type()) >= 0 && vp.scalar_type() == kp.scalar_type(), "the cache is bf16 or fp16");
+  need(table.dim() == 2 && table.scalar_type() == at::kInt && lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == table.size(0),
+       "table is int32 [B, width], lens int32 [B]");
+  need(kp.stride(3) == 1 && vp.stride(3) == 1 && table.stride(1) == 1 && lens.stride(0) == 1,
+       "the last dimensions of the cache, of table and of lens have to be contiguous");
+}
+int as_int(int64_t v) {
+  need(v >= 0 && v <= 0x7fffffff, "a size beyond 31 bits");
+  return (int)v;
+}
+
+// ------------------------------------------------------------------------------------------ append
+// (k, v, k_pages, v_pages, table, lens, q, cos, sin, starts, interleaved, stream) -> q rotated or None
+PyObject* append(PyObject* const* a) {
+  const at::Tensor &k = tensor(a[0]), &v = tensor(a[1]), &kp = tensor(a[2]), &vp = tensor(a[3]), &table = tensor(a[4]), &lens = tensor(a[5]);
+  const Maybe q = maybe(a[6]), cos = maybe(a[7]), sin = maybe(a[8]), starts = maybe(a[9]);
+  check_cache(kp, vp, table, lens);
+  const int64_t B = table.size(0), width = table.size(1), page = kp.size(1), hkv = kp.size(2), D = kp.size(3);
+  need(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == hkv && k.size(2) == D, "k and v are [T, kv_heads, D] with the cache's heads and D");
+  const int64_t T = k.size(0);
+  const at::ScalarType dt = kp.scalar_type();
+  need(k.scalar_type() == dt && v.scalar_type() == dt && k.stride(2) == 1 && v.stride(2) == 1,
+       "k and v have the cache's type and a contiguous last dimension");
+  need(D % 8 == 0, "D is a multiple of 8");
+  same_device(k.device(), {&v, &kp, &vp, &table, &lens, q.t, cos.t, sin.t, starts.t});
+  if (q)
+    need(q->dim() == 3 && q->size(0) == T && q->size(2) == D && q->scalar_type() == dt && q->stride(2) == 1,
+         "q is [T, heads, D] of the cache's type and device with a contiguous last dimension");
+  need((bool)cos == (bool)sin, "cos and sin come together");
+  int64_t rot = 0;
+  if (cos) {
+    need(cos->dim() == 2 && cos->sizes() == sin->sizes(), "cos and sin are [P, rot / 2] with P >= width * page, rot <= D and rot % 16 == 0");
+    rot = 2 * cos->size(1);
+    need(cos->size(0) >= width * page && rot <= D && rot % 16 == 0, "cos and sin are [P, rot / 2] with P >= width * page, rot <= D and rot % 16 == 0");
+    need(cos->scalar_type() == at::kFloat && sin->scalar_type() == at::kFloat && cos->is_contiguous() && sin->is_contiguous(),
+         "cos and sin are contiguous fp32");
+  }
+  if (starts)
+    need(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == B + 1 && starts->stride(0) == 1,
+         "starts is int32 [B + 1] on the cache's device");
+  else
+    need((B ? T % B : T) == 0, "without starts every sequence has the same number of new tokens");
+  const Where w(k, a[11]);
+  at::Tensor qo;
+  if (q) qo = B && width ? at::empty({T, q->size(1), D}, q->options()) : at::zeros({T, q->size(1), D}, q->options());
+  launched(k_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), q.ptr(), q ? q->stride(0) : 0,
+                    q ? q->stride(1) : 0, q ? qo.data_ptr() : nullptr, kp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2), vp.data_ptr(),
+                    vp.stride(0), vp.stride(1), vp.stride(2), table.data_ptr(), table.stride(0), lens.data_ptr(), starts.ptr(), cos.ptr(),
+                    sin.ptr(), as_int(B), as_int(T), q ? as_int(q->size(1)) : 0, as_int(hkv), as_int(D), (int)rot, as_int(page), as_int(width),
+                    as_int(kp.size(0)), truth(a[10]), half_type(dt), w.stream),
+           "dlamd_paged_append");
+  if (!q) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(qo));
+}
+
+// ------------------------------------------------------------------------------------------ attention
+struct Deal {
+  int64_t share, least;
+};
+// How a call's tiles of keys are dealt out: {0, 0}, a workgroup per problem (sequence, key head, group of rows), or workgroups to
+// deal all tiles out to and the least tiles of a part.
+//   * Up to a tile of keys there is nothing to split; 1024 sequence heads x 577 keys: 34.5 us one workgroup each, 37.7 us in
+//     parts (the join); 16 heads x 1000 keys: 9.4 and 8.3 us.
+//   * Otherwise as many workgroups as are resident at once by their registers (3 per compute unit up to 16 rows of D 128, 2
+//     beyond; 4 and 3 for D 64): 8 x 16384 keys, 8 heads of 128: 101 us with 768, 103 with 256.
+//   * A part's (m, l, o) costs rows x D floats written and read, so more rows make longer parts: 64 rows x 16384 keys: 27 us
+//     with 8 tiles at least, 29 with 16 and 2.
+Deal deal_out(int64_t problems, int64_t rows, int64_t bound, int64_t D) {
+  const int64_t tile = rows <= 32 ? 128 : 64;
+  if (bound <= tile || (problems >= 192 && bound <= 1024)) return {0, 0};
+  const int64_t resident = D == 64 ? (rows <= 16 ? 4 : 3) : (rows <= 16 ? 3 : 2);
+  return {256 * resident, std::max<int64_t>(1, 8 * rows / tile)};
+}
+
+// (q, k_pages, v_pages, table, lens, scale or None, causal, max_len or None, return_lse, share or None, least, stream)
+PyObject* attention(PyObject* const* a) {
+  const at::Tensor &q = tensor(a[0]), &kp = tensor(a[1]), &vp = tensor(a[2]), &table = tensor(a[3]), &lens = tensor(a[4]);
+  check_cache(kp, vp, table, lens);
+  need(q.dim() == 4 && q.scalar_type() == kp.scalar_type() && q.stride(3) == 1,
+       "q is [B, n, heads, D] of the cache's type with a contiguous last dimension");
+  const int64_t B = q.size(0), n = q.size(1), hq = q.size(2), D = q.size(3), page = kp.size(1), hkv = kp.size(2), width = table.size(1);
+  need(table.size(0) == B && kp.size(3) == D && hkv > 0 && hq % hkv == 0,
+       "q, table and cache disagree: one table row per sequence, D alike, heads a multiple of kv_heads");
+  need(page > 0 && page % 16 == 0 && (D == 64 || D == 128), "page is a multiple of 16, D is 64 or 128");
+  same_device(q.device(), {&kp, &vp, &table, &lens});
+  double scale = 1.0 / std::sqrt((double)D);
+  if (a[5] != Py_None) {
+    scale = PyFloat_AsDouble(a[5]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      throw Refused("scale is a number");
+    }
+  }
+  int64_t bound = width * page;
+  if (a[7] != Py_None) bound = std::min<int64_t>(bound, number(a[7]));
+  const int64_t rows = n * (hq / hkv), problems = B * hkv * ((rows + 63) / 64);
+  const Deal d = a[9] == Py_None ? deal_out(problems, rows, bound, D) : Deal{number(a[9]), number(a[10])};
+  const Where w(q, a[11]);
+  at::Tensor o = at::empty({B, n, hq, D}, q.options()), lse, part;
+  const bool want = truth(a[8]);
+  if (want) lse = at::empty({B, n, hq}, q.options().dtype(at::kFloat));
+  if (d.share) part = at::empty({d.share + problems, std::min<int64_t>(rows, 64), D + 4}, q.options().dtype(at::kFloat));
+  launched(k_attention(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), kp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
+                       vp.data_ptr(), vp.stride(0), vp.stride(1), vp.stride(2), table.data_ptr(), table.stride(0), lens.data_ptr(),
+                       o.data_ptr(), want ? lse.data_ptr() : nullptr, d.share ? part.data_ptr() : nullptr, as_int(d.share), as_int(d.least),
+                       as_int(B), as_int(n), as_int(hq), as_int(hkv), as_int(D), as_int(page), as_int(width), as_int(kp.size(0)), truth(a[6]),
+                       (float)scale, half_type(q.scalar_type()), w.stream),
+           "dlamd_paged_attention");
+  PyObject* po = THPVariable_Wrap(std::move(o));
+  if (!want) return po;
+  PyObject* pl = THPVariable_Wrap(std::move(lse));
+  return Py_BuildValue("(NN)", po, pl);
+}
+
+// ------------------------------------------------------------------------------------------ verification
+// Workgroups that share a row.  Up to 8192 tokens one holds the row in registers (8 x 4000: 5.8 us, 8.5 in pieces); a large
+// batch keeps the card busy by itself (192 x 50265: 24 us, 21.6 in 32 pieces with a second launch); 1 x 50265: 8.2 us in 48
+// pieces, 17.6 in one.
+int64_t pieces_of(int64_t B, int64_t V) {
+  if (V <= 8192 || B >= 128) return 1;
+  return B < 32 ? std::min<int64_t>(48, (V + 511) / 512) : std::min<int64_t>(32, (V + 2047) / 2048);
+}
+
+// (draft, target, u, proposal, counts, pad, pieces or None, stream) -> (tokens, accepted)
+PyObject* verify(PyObject* const* a) {
+  const at::Tensor &draft = tensor(a[0]), &target = tensor(a[1]), &u = tensor(a[2]);
+  const Maybe proposal = maybe(a[3]), counts = maybe(a[4]);
+  need(draft.dim() == 2 && draft.scalar_type() == at::kInt, "draft is int32 [B, n]");
+  const int64_t B = draft.size(0), n = draft.size(1);
+  need(n <= 63, "at most 63 drafted tokens");
+  const at::ScalarType dt = target.scalar_type();
+  const int type = dt == at::kFloat ? 2 : half_type(dt);
+  need(target.dim() == 3 && target.size(0) == B && target.size(1) == n + 1 && type >= 0 && target.size(2) > 0,
+       "target is [B, n + 1, V] bf16, fp16 or fp32");
+  const int64_t V = target.size(2);
+  if (proposal)
+    need(proposal->dim() == 3 && proposal->size(0) == B && proposal->size(1) == n && proposal->size(2) == V && proposal->scalar_type() == dt &&
+             proposal->stride(2) == 1,
+         "proposal is [B, n, V] of the target's type, rows contiguous");
+  need(u.dim() == 2 && u.size(0) == B && u.size(1) == n + 1 && u.scalar_type() == at::kFloat && u.stride(1) == 1, "u is fp32 [B, n + 1]");
+  if (counts) need(counts->dim() == 1 && counts->size(0) == B && counts->scalar_type() == at::kInt && counts->stride(0) == 1, "counts is int32 [B]");
+  need(target.stride(2) == 1 && draft.stride(1) == 1, "the last dimension of target and draft has to be contiguous");
+  same_device(draft.device(), {&target, &u, proposal.t, counts.t});
+  const ll pad = number(a[5]);
+  need(pad >= -0x80000000LL && pad <= 0x7fffffffLL, "pad is an int32");
+  const Where w(draft, a[7]);
+  at::Tensor tokens = at::empty({B, n + 1}, draft.options()), accepted = at::empty({B}, draft.options()), sums;
+  const int64_t pieces = a[6] == Py_None ? pieces_of(B, V) : number(a[6]);
+  if (pieces > 1) sums = at::empty({B, pieces, 2}, draft.options().dtype(at::kDouble));
+  const bool with_q = proposal && n > 0;
+  launched(k_verify(draft.data_ptr(), draft.stride(0), target.data_ptr(), target.stride(0), target.stride(1), with_q ? proposal.ptr() : nullptr,
+                    with_q ? proposal->stride(0) : 0, with_q ? proposal->stride(1) : 0, u.data_ptr(), u.stride(0), counts.ptr(),
+                    tokens.data_ptr(), accepted.data_ptr(), pieces > 1 ? sums.data_ptr() : nullptr, as_int(pieces), as_int(B), as_int(n),
+                    as_int(V), (int)pad, type, w.stream),
+           "dlamd_verify_draft");
+  PyObject* pt = THPVariable_Wrap(std::move(tokens));
+  PyObject* pa = THPVariable_Wrap(std::move(accepted));
+  return Py_BuildValue("(NN)", pt, pa);
+}
+
+// ------------------------------------------------------------------------------------------ 4-bit linear layer
+struct Shape {
+  int tiles, nw, kw, kz;                                     // tiles of 16 outputs per wave, waves over outputs and K, parts of K
+};
+Shape shape_of(int64_t M, int64_t N, int64_t K) {
+  const int steps = (int)std::min<int64_t>((K + 127) / 128, 1 << 20);
+  if (N < 8192) return {1, 1, std::min(8, steps), 1};
+  if (M <= 16) return {2, 1, std::min(4, steps), 1};
+  return {4, 1, std::min(4, steps), N < 10000 && steps >= 64 ? 2 : 1};
+}
+
+// (x, words, scale, zero, n, k, group, bias, act, res, shape or None, stream) -> y
+PyObject* int4(PyObject* const* a) {
+  const at::Tensor &x = tensor(a[0]), &words = tensor(a[1]), &scale = tensor(a[2]);
+  const Maybe zero = maybe(a[3]), bias = maybe(a[7]), res = maybe(a[9]);
+  const int64_t N = number(a[4]), K = number(a[5]), G = number(a[6]);
+  const int type = half_type(x.scalar_type());
+  const int64_t dims = x.dim();
+  need(dims > 0 && x.size(dims - 1) == K && type >= 0, "x is [..., K] bf16 or fp16");
+  if (bias) need(bias->dim() == 1 && bias->size(0) == N && bias->scalar_type() == at::kFloat && bias->stride(0) == 1, "bias is fp32 [N]");
+  if (res)
+    need(res->dim() == dims && res->size(dims - 1) == N && res->sizes().slice(0, dims - 1) == x.sizes().slice(0, dims - 1) &&
+             res->scalar_type() == x.scalar_type(),
+         "res is [..., N] of x's type");
+  same_device(x.device(), {&words, &scale, zero.t, bias.t, res.t});
+  const Where w(x, a[11]);
+  at::Tensor x2 = dims == 2 ? x : x.reshape({-1, K}), r2;
+  if (x2.stride(1) != 1 || x2.stride(0) % 8 != 0 || ((uintptr_t)x2.data_ptr() & 15))
+    x2 = x2.clone(at::MemoryFormat::Contiguous);             // rows the kernel cannot load 16 bytes at a time
+  if (res) {
+    r2 = dims == 2 ? *res.t : res->reshape({-1, N});
+    if (r2.stride(1) != 1) r2 = r2.contiguous();
+  }
+  const int64_t M = x2.size(0);
+  c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
+  sizes[dims - 1] = N;
+  at::Tensor y = at::empty(sizes, x.options()), part;
+  Shape s = shape_of(M, N, K);
+  if (a[10] != Py_None) {
+    need(PyTuple_Check(a[10]) && PyTuple_GET_SIZE(a[10]) == 4, "shape is (tiles, waves over outputs, waves over K, parts of K)");
+    s = {(int)number(PyTuple_GET_ITEM(a[10], 0)), (int)number(PyTuple_GET_ITEM(a[10], 1)), (int)number(PyTuple_GET_ITEM(a[10], 2)),
+         (int)number(PyTuple_GET_ITEM(a[10], 3))};
+  }
+  if (s.kz > 1) part = at::empty({s.kz, M, (N + 15) / 16 * 16}, x.options().dtype(at::kFloat));
+  launched(k_int4(x2.data_ptr(), x2.stride(0), words.data_ptr(), scale.data_ptr(), zero.ptr(), bias.ptr(), res ? r2.data_ptr() : nullptr,
+                  res ? r2.stride(0) : 0, y.data_ptr(), as_int(M), as_int(N), as_int(K), as_int(G), (int)number(a[8]), type,
+                  half_type(scale.scalar_type()), s.tiles, s.nw, s.kw, s.kz, s.kz > 1 ? part.data_ptr() : nullptr, w.stream),
+           "dlamd_int4_linear");
+  return THPVariable_Wrap(std::move(y));
+}
+
+// ------------------------------------------------------------------------------------------ module
+// No C++ exception leaves an entry: a refused argument is a ValueError, a kernel's code the framework's own error.
+template <PyObject* (*F)(PyObject* const*), int N>
+PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != N) {
+    PyErr_Format(PyExc_TypeError, "%d arguments are expected, %zd came", N, n);
+    return nullptr;
+  }
+  try {
+    return F(args);
+  } catch (const Refused& e) {
+    PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const Failed& e) {
+    PyErr_SetString(k_error ? k_error : PyExc_RuntimeError, e.what());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
+  }
+  return nullptr;
+}
+
+// (address of append, attention, verify, int4, error class)
+PyObject* init(PyObject* const* a) {
+  auto at = [&](int i) { return (void*)(intptr_t)number(a[i]); };
+  k_append = reinterpret_cast<decltype(k_append)>(at(0));
+  k_attention = reinterpret_cast<decltype(k_attention)>(at(1));
+  k_verify = reinterpret_cast<decltype(k_verify)>(at(2));
+  k_int4 = reinterpret_cast<decltype(k_int4)>(at(3));
+  Py_XINCREF(a[4]);
+  k_error = a[4];
+  Py_RETURN_NONE;
+}
+// (problems, rows, bound, D), (B, V), (M, N, K): the rules above, for tests
+PyObject* rule_deal(PyObject* const* a) {
+  const Deal d = deal_out(number(a[0]), number(a[1]), number(a[2]), number(a[3]));
+  return Py_BuildValue("(LL)", (ll)d.share, (ll)d.least);
+}
+PyObject* rule_pieces(PyObject* const* a) { return PyLong_FromLongLong(pieces_of(number(a[0]), number(a[1]))); }
+PyObject* rule_shape(PyObject* const* a) {
+  const Shape s = shape_of(number(a[0]), number(a[1]), number(a[2]));
+  return Py_BuildValue("(iiii)", s.tiles, s.nw, s.kw, s.kz);
+}
+
+#define ENTRY(name, f, n, doc) {name, (PyCFunction)(void*)entry<f, n>, METH_FASTCALL, doc}
+PyMethodDef methods[] = {
+    ENTRY("init", init, 5, "addresses of the kernels' C entries, the error class"),
+    ENTRY("paged_append", append, 12, "ops.paged.paged_append on device tensors"),
+    ENTRY("paged_attention", attention, 12, "ops.paged.paged_attention on device tensors"),
+    ENTRY("verify_draft", verify, 8, "ops.draft.verify_draft on device tensors"),
+    ENTRY("linear_int4", int4, 12, "ops.int4.linear_int4 on device tensors"),
+    ENTRY("rule_deal", rule_deal, 4, "how attention deals its work out"),
+    ENTRY("rule_pieces", rule_pieces, 2, "workgroups per row of a verification"),
+    ENTRY("rule_shape", rule_shape, 3, "launch shape of a 4-bit linear layer"),
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "dlamd_bind", "host side of the decode-step operators", -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_dlamd_bind() { return PyModule_Create(&module); }

@@ -10,6 +10,8 @@ raises instead of silently falling back to eager PyTorch.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -57,14 +59,29 @@ def stream_ptr() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 """Handle of the current stream of a device, by its index."""
 
+BIND_LIB = LIB_DIR / "dlamd_bind.so"
+_BIND = None
 
-def elsewhere(index: int) -> bool:
-    """Whether device ``index`` is not the current one (kernels launch on the current device: the caller then enters
-    ``torch.cuda.device(index)`` first)."""
-    return torch._C._cuda_getDevice() != index
+
+def bind():
+    """Load (once) the CPython module with the host side of the decode-step operators and give it the kernels' entries."""
+    global _BIND
+    if _BIND is None:
+        kernels = lib()
+        with _LOCK:
+            if _BIND is None:
+                if not BIND_LIB.exists():
+                    raise KernelLibraryError(f"{BIND_LIB} is missing: run `python -m distributed_llms_amd.utils.build`")
+                loader = importlib.machinery.ExtensionFileLoader("dlamd_bind", str(BIND_LIB))
+                m = importlib.util.module_from_spec(importlib.util.spec_from_loader("dlamd_bind", loader))
+                loader.exec_module(m)
+                names = ("dlamd_paged_append", "dlamd_paged_attention", "dlamd_verify_draft", "dlamd_int4_linear")
+                m.init(*(ctypes.cast(getattr(kernels, n), ctypes.c_void_p).value for n in names), KernelLibraryError)
+                _BIND = m
+    return _BIND
 
 
 def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
@@ -130,10 +147,5 @@ def _declare(l: ctypes.CDLL) -> None:
     sig("dlamd_dar_register", [vp, vp, ll, vp])
     sig("dlamd_dar_register_peer", [vp, i, i, vp])
     sig("dlamd_dar_allreduce_region", [vp, i, ll, i, f, i, vp])
-    sig("dlamd_paged_append", [vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, vp, vp, vp, vp]
-        + [i] * 11 + [vp])
-    sig("dlamd_paged_attention", [vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, ll, ll, vp, ll, vp, vp, vp, vp] + [i] * 11 + [f, i, vp])
-    sig("dlamd_verify_draft", [vp, ll, vp, ll, ll, vp, ll, ll, vp, ll, vp, vp, vp, vp] + [i] * 6 + [vp])
-    sig("dlamd_int4_linear", [vp, ll, vp, vp, vp, vp, vp, ll, vp] + [i] * 11 + [vp, vp])
     sig("dlamd_embed_rows", [vp, vp, vp, vp, vp, ll, i, i, i, i, f, vp])
     sig("dlamd_decode_bookkeep", [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp])

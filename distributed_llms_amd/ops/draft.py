@@ -1,4 +1,5 @@
-"""Verification of drafted tokens.  GPU: csrc/kernels/draft_verify.hip; CPU tensors: plain PyTorch (also the oracle).
+"""Verification of drafted tokens.  GPU: csrc/kernels/draft_verify.hip through csrc/bind/decode_ops.cpp; CPU
+tensors: plain PyTorch (also the oracle).
 
 A cheap proposal drafts n tokens, the target model scores all of them in one pass, and ``verify_draft`` keeps the longest
 prefix the target agrees with plus one token of the target's own - so that the kept tokens are distributed exactly as if
@@ -11,7 +12,6 @@ import torch
 
 from . import _loader
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_DRAFTED = 63
 
 
@@ -57,11 +57,15 @@ def verify_draft_reference(draft, target, u, proposal=None, counts=None, pad: in
     return tokens.to(draft.device), accepted.to(draft.device)
 
 
-def _pieces(B: int, V: int) -> int:
-    """Workgroups that share a row."""
-    if V <= 8192 or B >= 128:
-        return 1
-    return min(48, -(-V // 512)) if B < 32 else min(32, -(-V // 2048))
+_PIECES: Optional[int] = None
+"""Workgroups per row in place of the rule in csrc/bind/decode_ops.cpp: for tests and sweeps."""
+_BIND = None
+
+
+def _bind():
+    global _BIND
+    _BIND = _loader.bind()
+    return _BIND
 
 
 def verify_draft(draft: torch.Tensor, target: torch.Tensor, u: torch.Tensor, proposal: Optional[torch.Tensor] = None,
@@ -79,16 +83,17 @@ def verify_draft(draft: torch.Tensor, target: torch.Tensor, u: torch.Tensor, pro
     Sampling takes the lowest v whose cumulative weight exceeds u times the row's total, in 64 bits.  Rows need not sum to
     one.  A drafted token outside [0, V) is refused.  Where nothing remains (target <= proposal everywhere) the target's
     row is sampled itself; a row without positive finite weight gives token 0."""
+    if draft.is_cuda:
+        return (_BIND or _bind()).verify_draft(draft, target, u, proposal, counts, pad, _PIECES, _loader.raw_stream(draft.get_device()))
     if draft.dim() != 2 or draft.dtype != torch.int32:
         raise ValueError("draft is int32 [B, n]")
     B, n = draft.shape
     dt = target.dtype
     if n > MAX_DRAFTED:
         raise ValueError(f"at most {MAX_DRAFTED} drafted tokens")
-    if target.dim() != 3 or target.shape[:2] != (B, n + 1) or dt not in _DTYPES or target.shape[2] == 0:
+    if target.dim() != 3 or target.shape[:2] != (B, n + 1) or dt not in (torch.bfloat16, torch.float16, torch.float32) or target.shape[2] == 0:
         raise ValueError("target is [B, n + 1, V] bf16, fp16 or fp32")
-    V = target.shape[2]
-    if proposal is not None and (proposal.shape != (B, n, V) or proposal.dtype != dt or proposal.stride(2) != 1):
+    if proposal is not None and (proposal.shape != (B, n, target.shape[2]) or proposal.dtype != dt or proposal.stride(2) != 1):
         raise ValueError("proposal is [B, n, V] of the target's type, rows contiguous")
     if u.shape != (B, n + 1) or u.dtype != torch.float32 or u.stride(1) != 1:
         raise ValueError("u is fp32 [B, n + 1]")
@@ -96,28 +101,6 @@ def verify_draft(draft: torch.Tensor, target: torch.Tensor, u: torch.Tensor, pro
         raise ValueError("counts is int32 [B]")
     if target.stride(2) != 1 or draft.stride(1) != 1:
         raise ValueError("the last dimension of target and draft has to be contiguous")
-    dev = draft.get_device()
-    if (target.get_device() != dev or u.get_device() != dev or (proposal is not None and proposal.get_device() != dev)
-            or (counts is not None and counts.get_device() != dev)):
+    if any(x is not None and x.device != draft.device for x in (target, u, proposal, counts)):
         raise ValueError("all tensors live on one device")
-    if dev < 0:
-        return verify_draft_reference(draft, target, u, proposal, counts, pad)
-    if _loader.elsewhere(dev):
-        with torch.cuda.device(dev):
-            return verify_draft(draft, target, u, proposal, counts, pad)
-    tokens = draft.new_empty((B, n + 1))
-    accepted = draft.new_empty((B,))
-    q_p = q_bs = q_ns = 0
-    if proposal is not None and n:
-        q_p = proposal.data_ptr()
-        q_bs, q_ns, _ = proposal.stride()
-    p_bs, p_ns, _ = target.stride()
-    pieces = _pieces(B, V)
-    sums = draft.new_empty((B, pieces, 2), dtype=torch.float64) if pieces > 1 else None
-    rc = _loader.lib().dlamd_verify_draft(
-        draft.data_ptr(), draft.stride(0), target.data_ptr(), p_bs, p_ns, q_p, q_bs, q_ns, u.data_ptr(), u.stride(0),
-        0 if counts is None else counts.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), 0 if sums is None else sums.data_ptr(),
-        pieces, B, n, V, pad, _DTYPES[dt], _loader.raw_stream(dev))
-    if rc:
-        _loader.check(rc, "dlamd_verify_draft")
-    return tokens, accepted
+    return verify_draft_reference(draft, target, u, proposal, counts, pad)

@@ -1,5 +1,5 @@
-"""Linear layers with 4-bit weights and group scales, for the few rows of a decode step.  GPU: csrc/kernels/int4_linear.hip;
-CPU tensors: plain PyTorch fp32 on the dequantized weights (also the oracle).
+"""Linear layers with 4-bit weights and group scales, for the few rows of a decode step.  GPU: csrc/kernels/int4_linear.hip
+through csrc/bind/decode_ops.cpp; CPU tensors: plain PyTorch fp32 on the dequantized weights (also the oracle).
 
 ``quantize_int4`` (from a float weight) or ``pack_int4`` (from codes, scales and zeros made elsewhere) lays a layer's weights
 out once; ``linear_int4`` is then called like ``ops.conv.linear_bf16``.  Weight (n, k) is (code - zero) * scale with codes
@@ -14,7 +14,6 @@ import torch
 from . import _loader
 from .conv import _act_ref
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _ACTS = {"none": 0, "relu": 1, "gelu": 3}
 GROUPS = (32, 64, 128)
 
@@ -61,7 +60,7 @@ def pack_int4(packed: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Te
     G = K // groups if groups else 0
     if N == 0 or G not in GROUPS or G * groups != K:
         raise ValueError("K is a multiple of the group size, which is 32, 64 or 128")
-    if scale.dtype not in _DTYPES:
+    if scale.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("scales are bf16 or fp16")
     if zero is not None and (zero.shape != scale.shape or zero.dtype != torch.uint8):
         raise ValueError("zero is uint8 of the scales' shape")
@@ -104,57 +103,34 @@ def linear_int4_reference(x, w: Int4Weight, bias=None, act: str = "none", res=No
     return _act_ref(y, act)
 
 
-def _shape(M: int, N: int, K: int):
-    """(tiles of 16 outputs a wave holds, waves over outputs, waves over K, parts of K over workgroups)."""
-    steps = -(-K // 128)
-    if N < 8192:
-        return 1, 1, min(8, steps), 1
-    if M <= 16:
-        return 2, 1, min(4, steps), 1
-    return 4, 1, min(4, steps), 2 if N < 10000 and steps >= 64 else 1
+_SHAPE = None
+"""(tiles of 16 outputs a wave holds, waves over outputs, waves over K, parts of K over workgroups) in place of the rule in
+csrc/bind/decode_ops.cpp: for tests and sweeps."""
+_BIND = None
+
+
+def _bind():
+    global _BIND
+    _BIND = _loader.bind()
+    return _BIND
 
 
 def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None, *, act: str = "none",
                 res: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = act(x @ W^T + bias (+ res)) in x's type.  x: [..., K] bf16 or fp16, bias: fp32 [N], res: [..., N] of x's type;
     act: none, relu, gelu.  Products are exact and summed in fp32, rounded once."""
-    if act not in _ACTS:
+    code = _ACTS.get(act)
+    if code is None:
         raise ValueError("act is none, relu or gelu")
-    N, K = w.n, w.k
-    if x.dim() == 0 or x.shape[-1] != K or x.dtype not in _DTYPES:
+    if x.is_cuda:
+        return (_BIND or _bind()).linear_int4(x, w.words, w.scale, w.zero, w.n, w.k, w.group, bias, code, res, _SHAPE,
+                                              _loader.raw_stream(x.get_device()))
+    if x.dim() == 0 or x.shape[-1] != w.k or x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("x is [..., K] bf16 or fp16")
-    if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or bias.stride(0) != 1):
+    if bias is not None and (bias.shape != (w.n,) or bias.dtype != torch.float32 or bias.stride(0) != 1):
         raise ValueError("bias is fp32 [N]")
-    if res is not None and (res.shape[:-1] != x.shape[:-1] or res.shape[-1] != N or res.dtype != x.dtype):
+    if res is not None and (res.shape[:-1] != x.shape[:-1] or res.shape[-1] != w.n or res.dtype != x.dtype):
         raise ValueError("res is [..., N] of x's type")
-    dev = x.get_device()
-    if w.words.get_device() != dev or (bias is not None and bias.get_device() != dev) or (res is not None and res.get_device() != dev):
+    if any(t is not None and t.device != x.device for t in (w.words, bias, res)):
         raise ValueError("all tensors live on one device")
-    if dev < 0:
-        return linear_int4_reference(x, w, bias, act, res).to(x.dtype)
-    if _loader.elsewhere(dev):
-        with torch.cuda.device(dev):
-            return linear_int4(x, w, bias, act=act, res=res)
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    x_rs, x_ks = x2.stride()
-    if x_ks != 1 or x_rs % 8 != 0 or x2.data_ptr() % 16 != 0:
-        # rows the kernel cannot load 16 bytes at a time
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-        x_rs = K
-    M = x2.shape[0]
-    r2_p = r_rs = 0
-    if res is not None:
-        r2 = res if res.dim() == 2 else res.reshape(-1, N)
-        if r2.stride(1) != 1:
-            r2 = r2.contiguous()
-        r2_p, r_rs = r2.data_ptr(), r2.stride(0)
-    y = x.new_empty((*x.shape[:-1], N))
-    tiles, nw, kw, kz = _shape(M, N, K)
-    part = x.new_empty((kz, M, -(-N // 16) * 16), dtype=torch.float32) if kz > 1 else None
-    rc = _loader.lib().dlamd_int4_linear(
-        x2.data_ptr(), x_rs, w.words.data_ptr(), w.scale.data_ptr(), 0 if w.zero is None else w.zero.data_ptr(),
-        0 if bias is None else bias.data_ptr(), r2_p, r_rs, y.data_ptr(), M, N, K, w.group, _ACTS[act], _DTYPES[x.dtype],
-        _DTYPES[w.scale.dtype], tiles, nw, kw, kz, 0 if part is None else part.data_ptr(), _loader.raw_stream(dev))
-    if rc:
-        _loader.check(rc, "dlamd_int4_linear")
-    return y
+    return linear_int4_reference(x, w, bias, act, res).to(x.dtype)

@@ -1,6 +1,6 @@
 """Paged key / value cache of a decoder: appending new tokens (with the position rotation on the way) and attention of one
-or a few new tokens per sequence over the cache.  GPU: csrc/kernels/paged_append.hip, csrc/kernels/paged_attention.hip;
-CPU tensors: plain PyTorch fp32 (also the oracle in tests).
+or a few new tokens per sequence over the cache.  GPU: csrc/kernels/paged_append.hip, csrc/kernels/paged_attention.hip
+through csrc/bind/decode_ops.cpp; CPU tensors: plain PyTorch fp32 (also the oracle in tests).
 
 The cache of a layer is two tensors ``k_pages``, ``v_pages`` [pages, page, kv_heads, D] (bf16 or fp16; views of one
 buffer are fine as long as D is contiguous and strides are multiples of 8).  Sequence ``b`` keeps position ``p`` in slot
@@ -28,7 +28,13 @@ import torch
 
 from . import _loader
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_BIND = None
+
+
+def _bind():
+    global _BIND
+    _BIND = _loader.bind()
+    return _BIND
 
 
 def rope_tables(positions: int, rot: int, base: float = 10000.0,
@@ -83,7 +89,7 @@ def paged_append_reference(k, v, k_pages, v_pages, table, lens, q=None, cos=None
 def _check_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor) -> None:
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError("k_pages and v_pages are [pages, page, kv_heads, D] of one shape")
-    if k_pages.dtype not in _DTYPES or v_pages.dtype != k_pages.dtype:
+    if k_pages.dtype not in (torch.bfloat16, torch.float16) or v_pages.dtype != k_pages.dtype:
         raise ValueError("the cache is bf16 or fp16")
     if table.dtype != torch.int32 or lens.dtype != torch.int32 or table.dim() != 2 or lens.shape != table.shape[:1]:
         raise ValueError("table is int32 [B, width], lens int32 [B]")
@@ -104,61 +110,36 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     (2 d, 2 d + 1).  ``q`` [T, heads, D]: the queries of the same tokens, rotated alike and returned as a new tensor
     (zeros for tokens of nobody, of idle rows and beyond the table); ``q`` itself is left as it is.  Dimensions of k, v
     and q may be strided (slices of a fused projection), the last one contiguous.  D % 8 == 0, rot % 16 == 0."""
+    if k.is_cuda:
+        return (_BIND or _bind()).paged_append(k, v, k_pages, v_pages, table, lens, q, cos, sin, starts, interleaved,
+                                               _loader.raw_stream(k.get_device()))
     _check_cache(k_pages, v_pages, table, lens)
     B, width = table.shape
-    pages, page, hkv, D = k_pages.shape
-    dt, dev = k_pages.dtype, k_pages.get_device()
-    shape = k.shape
-    if len(shape) != 3 or shape != v.shape or shape[1] != hkv or shape[2] != D:
+    page, hkv, D = k_pages.shape[1:]
+    dt = k_pages.dtype
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != hkv or k.shape[2] != D:
         raise ValueError("k and v are [T, kv_heads, D] with the cache's heads and D")
-    T = shape[0]
-    k_ts, k_hs, k_ds = k.stride()
-    v_ts, v_hs, v_ds = v.stride()
-    if k.dtype != dt or v.dtype != dt or k_ds != 1 or v_ds != 1:
+    T = k.shape[0]
+    if k.dtype != dt or v.dtype != dt or k.stride(2) != 1 or v.stride(2) != 1:
         raise ValueError("k and v have the cache's type and a contiguous last dimension")
     if D % 8 != 0:
         raise ValueError("D is a multiple of 8")
-    if k.get_device() != dev or v.get_device() != dev or v_pages.get_device() != dev or table.get_device() != dev or lens.get_device() != dev:
+    if any(x is not None and x.device != k.device for x in (v, k_pages, v_pages, table, lens, q, cos, sin, starts)):
         raise ValueError("all tensors live on one device")
-    hq = q_ts = q_hs = rot = cos_p = sin_p = starts_p = 0
-    if q is not None:
-        if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != dt or q.stride(2) != 1 or q.get_device() != dev:
-            raise ValueError("q is [T, heads, D] of the cache's type and device with a contiguous last dimension")
-        hq = q.shape[1]
-        q_ts, q_hs, _ = q.stride()
-    if cos is not None or sin is not None:
-        if cos is None or sin is None:
-            raise ValueError("cos and sin come together")
+    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != dt or q.stride(2) != 1):
+        raise ValueError("q is [T, heads, D] of the cache's type and device with a contiguous last dimension")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if cos is not None:
         rot = 2 * cos.shape[-1]
         if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < width * page or rot > D or rot % 16 != 0:
             raise ValueError("cos and sin are [P, rot / 2] with P >= width * page, rot <= D and rot % 16 == 0")
-        if cos.get_device() != dev or sin.get_device() != dev:
-            raise ValueError("all tensors live on one device")
-        if dev >= 0 and (cos.dtype != torch.float32 or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()):
-            raise ValueError("cos and sin are contiguous fp32")
-        cos_p, sin_p = cos.data_ptr(), sin.data_ptr()
     if starts is not None:
-        if starts.dtype != torch.int32 or starts.shape != (B + 1,) or starts.stride(0) != 1 or starts.get_device() != dev:
+        if starts.dtype != torch.int32 or starts.shape != (B + 1,) or starts.stride(0) != 1:
             raise ValueError("starts is int32 [B + 1] on the cache's device")
-        starts_p = starts.data_ptr()
     elif (T % B if B else T) != 0:
         raise ValueError("without starts every sequence has the same number of new tokens")
-    if dev < 0:
-        return paged_append_reference(k, v, k_pages, v_pages, table, lens, q, cos, sin, starts, interleaved)
-    if _loader.elsewhere(dev):
-        with torch.cuda.device(dev):
-            return paged_append(k, v, k_pages, v_pages, table, lens, q, cos, sin, starts, interleaved)
-    qo = None if q is None else (q.new_empty if B and width else q.new_zeros)((T, hq, D))
-    kp_ps, kp_ss, kp_hs, _ = k_pages.stride()
-    vp_ps, vp_ss, vp_hs, _ = v_pages.stride()
-    rc = _loader.lib().dlamd_paged_append(
-        k.data_ptr(), k_ts, k_hs, v.data_ptr(), v_ts, v_hs, 0 if q is None else q.data_ptr(), q_ts, q_hs,
-        0 if q is None else qo.data_ptr(), k_pages.data_ptr(), kp_ps, kp_ss, kp_hs, v_pages.data_ptr(), vp_ps, vp_ss, vp_hs,
-        table.data_ptr(), table.stride(0), lens.data_ptr(), starts_p, cos_p, sin_p, B, T, hq, hkv, D, rot, page, width, pages,
-        1 if interleaved else 0, _DTYPES[dt], _loader.raw_stream(dev))
-    if rc:
-        _loader.check(rc, "dlamd_paged_append")
-    return qo
+    return paged_append_reference(k, v, k_pages, v_pages, table, lens, q, cos, sin, starts, interleaved)
 
 
 def paged_attention_reference(q, k_pages, v_pages, table, lens, scale: Optional[float] = None, causal: bool = True,
@@ -188,17 +169,9 @@ def paged_attention_reference(q, k_pages, v_pages, table, lens, scale: Optional[
     return o, lse
 
 
-def _share(problems: int, rows: int, bound: int, D: int) -> Tuple[int, int]:
-    """How a call's work is dealt out: (0, 0), a workgroup per problem (sequence, key head, group of rows), or (workgroups to
-    deal all tiles of keys out to, least tiles of a part)."""
-    tile = 128 if rows <= 32 else 64
-    if bound <= tile or (problems >= 192 and bound <= 1024):
-        return 0, 0
-    return 256 * (_RESIDENT[D][0] if rows <= 16 else _RESIDENT[D][1]), max(1, 8 * rows // tile)
-
-
-# workgroups of the kernel that are resident on a compute unit (by its registers): rows <= 16, more
-_RESIDENT = {64: (4, 3), 128: (3, 2)}
+_DEAL: Tuple[Optional[int], int] = (None, 0)
+"""(workgroups to deal all tiles out to, least tiles of a part) in place of the rule in csrc/bind/decode_ops.cpp: for tests and
+sweeps."""
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
@@ -213,42 +186,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (cross-attention over encoder tokens held in pages).  A query that sees nothing gives 0 and a log-sum-exp of -inf.
     ``max_len``: an upper bound of the positions any query sees, when the caller knows a tighter one than ``width * page``
     (only used to choose how the work is split; lengths are read on the device).  D is 64 or 128, page % 16 == 0."""
+    if q.is_cuda:
+        return (_BIND or _bind()).paged_attention(q, k_pages, v_pages, table, lens, scale, causal, max_len, return_lse, *_DEAL,
+                                                  _loader.raw_stream(q.get_device()))
     _check_cache(k_pages, v_pages, table, lens)
-    if q.dim() != 4 or q.dtype != k_pages.dtype:
+    if q.dim() != 4 or q.dtype != k_pages.dtype or q.stride(3) != 1:
         raise ValueError("q is [B, n, heads, D] of the cache's type with a contiguous last dimension")
     B, n, hq, D = q.shape
-    q_bs, q_ns, q_hs, q_ds = q.stride()
-    pages, page, hkv, kD = k_pages.shape
-    width, dev = table.shape[1], q.get_device()
-    if q_ds != 1:
-        raise ValueError("q is [B, n, heads, D] of the cache's type with a contiguous last dimension")
+    page, hkv, kD = k_pages.shape[1:]
     if table.shape[0] != B or kD != D or hkv == 0 or hq % hkv != 0:
         raise ValueError("q, table and cache disagree: one table row per sequence, D alike, heads a multiple of kv_heads")
-    if page % 16 != 0 or page == 0 or (D != 64 and D != 128):
+    if page % 16 != 0 or page == 0 or D not in (64, 128):
         raise ValueError("page is a multiple of 16, D is 64 or 128")
-    if k_pages.get_device() != dev or v_pages.get_device() != dev or table.get_device() != dev or lens.get_device() != dev:
+    if any(x.device != q.device for x in (k_pages, v_pages, table, lens)):
         raise ValueError("all tensors live on one device")
-    scale = D ** -0.5 if scale is None else float(scale)
-    if dev < 0:
-        o, lse = paged_attention_reference(q, k_pages, v_pages, table, lens, scale, causal)
-        return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)
-    if _loader.elsewhere(dev):
-        with torch.cuda.device(dev):
-            return paged_attention(q, k_pages, v_pages, table, lens, scale, causal, max_len, return_lse)
-    o = q.new_empty((B, n, hq, D))
-    lse = q.new_empty((B, n, hq), dtype=torch.float32) if return_lse else None
-    rows = n * (hq // hkv)
-    problems = B * hkv * -(-rows // 64)
-    bound = width * page
-    share, least = _share(problems, rows, bound if max_len is None else min(max_len, bound), D)
-    part = q.new_empty((share + problems, min(rows, 64), D + 4), dtype=torch.float32) if share else None
-    kp_ps, kp_ss, kp_hs, _ = k_pages.stride()
-    vp_ps, vp_ss, vp_hs, _ = v_pages.stride()
-    rc = _loader.lib().dlamd_paged_attention(
-        q.data_ptr(), q_bs, q_ns, q_hs, k_pages.data_ptr(), kp_ps, kp_ss, kp_hs, v_pages.data_ptr(), vp_ps, vp_ss, vp_hs,
-        table.data_ptr(), table.stride(0), lens.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        0 if part is None else part.data_ptr(), share, least, B, n, hq, hkv, D, page, width, pages, 1 if causal else 0, scale,
-        _DTYPES[q.dtype], _loader.raw_stream(dev))
-    if rc:
-        _loader.check(rc, "dlamd_paged_attention")
-    return (o, lse) if return_lse else o
+    o, lse = paged_attention_reference(q, k_pages, v_pages, table, lens, scale, causal)
+    return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)

@@ -8,6 +8,9 @@ gfx950 only:
   kernels launch on the HIP stream PyTorch-ROCm is currently using)
 * ``csrc/pdf/*.cpp``      -> ``distributed_llms_amd/_lib/libdlamd_pdf.so``
   (C++ PDF reader / classifier / JPEG tools; host only)
+* ``csrc/bind/*.cpp``     -> ``distributed_llms_amd/_lib/dlamd_bind.so``
+  (CPython module against PyTorch's headers: the host side of the operators
+  whose kernels are shorter than a Python call; it launches through the C ABI)
 * ``csrc/runtime/*.cpp``  -> ``distributed_llms_amd/_lib/libdlamd_runtime.so``
   (C++ batcher, shared-memory page ring, host thread pool)
 
@@ -154,9 +157,33 @@ def build_runtime(force: bool = False, jobs: int = 8, verbose: bool = False) -> 
     return _build_cpp("runtime", "runtime", ["-lrt"], force, jobs, verbose)
 
 
+def build_bind(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the CPython module of csrc/bind against the installed PyTorch (host code only)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+
+    srcs = sorted((CSRC / "bind").glob("*.cpp"))
+    out = LIB_DIR / "dlamd_bind.so"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    digest = _sha(srcs, " ".join(flags) + torch.__version__ + sys.version)
+    if not force and _up_to_date("bind", digest, out):
+        return out
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    inc = [f"-I{p}" for p in [*ext.include_paths(), sysconfig.get_paths()["include"]]]
+    libs = [f"-L{p}" for p in ext.library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+    _run([CXX, *flags, *inc, "-shared", "-o", str(out), *map(str, srcs), *libs])
+    _stamp_path("bind").write_text(json.dumps({"digest": digest}))
+    if verbose:
+        print(f"[build] {out} ({len(srcs)} C++ sources)")
+    return out
+
+
 def build_all(force: bool = False, jobs: int = 8, verbose: bool = False) -> Dict[str, Path]:
     out = {}
     out["kernels"] = build_kernels(force, jobs, verbose)
+    out["bind"] = build_bind(force, verbose)
     if (CSRC / "pdf").exists() and any((CSRC / "pdf").glob("*.cpp")):
         out["pdf"] = build_pdf(force, jobs, verbose)
     if (CSRC / "runtime").exists() and any((CSRC / "runtime").glob("*.cpp")):

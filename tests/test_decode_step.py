@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from distributed_llms_amd.models.trocr import TrOCR, TrOCRConfig
+from distributed_llms_amd.ops import _loader
 from distributed_llms_amd.ops import draft as D
 from distributed_llms_amd.ops import int4 as Q
 from distributed_llms_amd.ops import paged as P
@@ -159,7 +160,8 @@ def test_two_streams_at_once():
         y = Q.linear_int4(s["x"], w)
         return (o, lse, y, *D.verify_draft(s["draft"], s["p"], s["u"]))
 
-    assert Q._shape(20, 9000, 8192)[3] > 1 and P._share(4, 24, 4096, 128)[0] and D._pieces(3, 40000) > 1
+    rules = _loader.bind()
+    assert rules.rule_shape(20, 9000, 8192)[3] > 1 and rules.rule_deal(4, 24, 4096, 128)[0] and rules.rule_pieces(3, 40000) > 1
     alone = [work(s) for s in sets]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in sets]

@@ -360,7 +360,7 @@ def test_attention_kernel_shares(case, share, least, monkeypatch):
     kept, n, page, hq, hkv, D, dt, causal, layout = ATT[case]
     c = att_case(case, kept, n, page, hq, hkv, D, DTYPES[dt], causal, layout)
     d = {x: on_gpu_with_strides(y) if torch.is_tensor(y) else y for x, y in c.items()}
-    monkeypatch.setattr(P, "_share", lambda *_: (share, least))
+    monkeypatch.setattr(P, "_DEAL", (share, least))
     o, lse = P.paged_attention(**d, return_lse=True)
     check_attention(c, o.cpu(), lse.cpu())
 
