@@ -11,6 +11,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include "../kernels/decode_abi.h"
+
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
@@ -35,14 +37,10 @@ void launched(int rc, const char* name) {
     throw Failed(std::string(name) + " failed with code " + std::to_string(rc) + " (host-side shape contract or launch error)");
 }
 
-int (*k_append)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, void*, void*, ll, ll, ll, void*, ll, ll, ll, const void*, ll,
-                const void*, const void*, const void*, const void*, int, int, int, int, int, int, int, int, int, int, int, void*);
-int (*k_attention)(const void*, ll, ll, ll, const void*, ll, ll, ll, const void*, ll, ll, ll, const void*, ll, const void*, void*, void*, void*,
-                   int, int, int, int, int, int, int, int, int, int, int, float, int, void*);
-int (*k_verify)(const void*, ll, const void*, ll, ll, const void*, ll, ll, const void*, ll, const void*, void*, void*, void*, int, int, int, int,
-                int, int, void*);
-int (*k_int4)(const void*, ll, const void*, const void*, const void*, const void*, const void*, ll, void*, int, int, int, int, int, int, int, int,
-              int, int, int, void*, void*);
+decltype(&dlamd_paged_append) k_append;
+decltype(&dlamd_paged_attention) k_attention;
+decltype(&dlamd_verify_draft) k_verify;
+decltype(&dlamd_int4_linear) k_int4;
 PyObject* k_error = nullptr;                                 // the framework's KernelLibraryError
 
 // ------------------------------------------------------------------------------------------ arguments
@@ -74,8 +72,8 @@ bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
 // Device of the call, made current for the launch, and its current stream as Python knows it.
 struct Where {
   c10::DeviceGuard guard;
-  void* stream;
-  Where(const at::Tensor& t, PyObject* s) : guard(t.device()), stream((void*)(intptr_t)number(s)) {}
+  ihipStream_t* stream;
+  Where(const at::Tensor& t, PyObject* s) : guard(t.device()), stream((ihipStream_t*)(intptr_t)number(s)) {}
 };
 void same_device(const c10::Device& d, std::initializer_list<const at::Tensor*> ts) {
   for (const at::Tensor* t : ts) need(!t || t->device() == d, "all tensors live on one device");
@@ -148,15 +146,13 @@ struct Deal {
 // deal all tiles out to and the least tiles of a part.
 //   * Up to a tile of keys there is nothing to split; 1024 sequence heads x 577 keys: 34.5 us one workgroup each, 37.7 us in
 //     parts (the join); 16 heads x 1000 keys: 9.4 and 8.3 us.
-//   * Otherwise as many workgroups as are resident at once by their registers (3 per compute unit up to 16 rows of D 128, 2
-//     beyond; 4 and 3 for D 64): 8 x 16384 keys, 8 heads of 128: 101 us with 768, 103 with 256.
-//   * A part's (m, l, o) costs rows x D floats written and read, so more rows make longer parts: 64 rows x 16384 keys: 27 us
-//     with 8 tiles at least, 29 with 16 and 2.
+//   * Otherwise as many workgroups as are resident at once by their registers, 3 per compute unit for D 128, 4 for D 64:
+//     8 x 16384 keys, 8 heads of 128: 101 us with 768, 103 with 256.
+//   * A part's (m, l, o) costs rows x D floats written and read: beyond 16 rows one workgroup per compute unit.  2 x 16384 keys,
+//     64 rows: 26.6 us with 256, 29.7 with 512; 12 ragged caches of up to 8009 keys, 40 rows: 26 and 34.
 Deal deal_out(int64_t problems, int64_t rows, int64_t bound, int64_t D) {
-  const int64_t tile = rows <= 32 ? 128 : 64;
-  if (bound <= tile || (problems >= 192 && bound <= 1024)) return {0, 0};
-  const int64_t resident = D == 64 ? (rows <= 16 ? 4 : 3) : (rows <= 16 ? 3 : 2);
-  return {256 * resident, std::max<int64_t>(1, 8 * rows / tile)};
+  if (bound <= 128 || (problems >= 192 && bound <= 1024)) return {0, 0};
+  return {rows > 16 ? 256 : D == 64 ? 1024 : 768, 1};
 }
 
 // (q, k_pages, v_pages, table, lens, scale or None, causal, max_len or None, return_lse, share or None, least, stream)
@@ -180,16 +176,17 @@ PyObject* attention(PyObject* const* a) {
   }
   int64_t bound = width * page;
   if (a[7] != Py_None) bound = std::min<int64_t>(bound, number(a[7]));
-  const int64_t rows = n * (hq / hkv), problems = B * hkv * ((rows + 63) / 64);
+  const int64_t all = n * (hq / hkv), groups = all <= 48 ? 1 : (all + 31) / 32, rows = (all + groups - 1) / groups;
+  const int64_t problems = B * hkv * groups;
   const Deal d = a[9] == Py_None ? deal_out(problems, rows, bound, D) : Deal{number(a[9]), number(a[10])};
   const Where w(q, a[11]);
   at::Tensor o = at::empty({B, n, hq, D}, q.options()), lse, part;
   const bool want = truth(a[8]);
   if (want) lse = at::empty({B, n, hq}, q.options().dtype(at::kFloat));
-  if (d.share) part = at::empty({d.share + problems, std::min<int64_t>(rows, 64), D + 4}, q.options().dtype(at::kFloat));
+  if (d.share) part = at::empty({d.share + problems, rows, D + 4}, q.options().dtype(at::kFloat));
   launched(k_attention(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), kp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
                        vp.data_ptr(), vp.stride(0), vp.stride(1), vp.stride(2), table.data_ptr(), table.stride(0), lens.data_ptr(),
-                       o.data_ptr(), want ? lse.data_ptr() : nullptr, d.share ? part.data_ptr() : nullptr, as_int(d.share), as_int(d.least),
+                       o.data_ptr(), want ? lse.data_ptr() : nullptr, d.share ? part.data_ptr() : nullptr, d.share ? part.numel() : 0, as_int(d.share), as_int(d.least),
                        as_int(B), as_int(n), as_int(hq), as_int(hkv), as_int(D), as_int(page), as_int(width), as_int(kp.size(0)), truth(a[6]),
                        (float)scale, half_type(q.scalar_type()), w.stream),
            "dlamd_paged_attention");
@@ -237,7 +234,7 @@ PyObject* verify(PyObject* const* a) {
   const bool with_q = proposal && n > 0;
   launched(k_verify(draft.data_ptr(), draft.stride(0), target.data_ptr(), target.stride(0), target.stride(1), with_q ? proposal.ptr() : nullptr,
                     with_q ? proposal->stride(0) : 0, with_q ? proposal->stride(1) : 0, u.data_ptr(), u.stride(0), counts.ptr(),
-                    tokens.data_ptr(), accepted.data_ptr(), pieces > 1 ? sums.data_ptr() : nullptr, as_int(pieces), as_int(B), as_int(n),
+                    tokens.data_ptr(), accepted.data_ptr(), pieces > 1 ? sums.data_ptr() : nullptr, pieces > 1 ? sums.numel() : 0, as_int(pieces), as_int(B), as_int(n),
                     as_int(V), (int)pad, type, w.stream),
            "dlamd_verify_draft");
   PyObject* pt = THPVariable_Wrap(std::move(tokens));
@@ -291,7 +288,7 @@ PyObject* int4(PyObject* const* a) {
   if (s.kz > 1) part = at::empty({s.kz, M, (N + 15) / 16 * 16}, x.options().dtype(at::kFloat));
   launched(k_int4(x2.data_ptr(), x2.stride(0), words.data_ptr(), scale.data_ptr(), zero.ptr(), bias.ptr(), res ? r2.data_ptr() : nullptr,
                   res ? r2.stride(0) : 0, y.data_ptr(), as_int(M), as_int(N), as_int(K), as_int(G), (int)number(a[8]), type,
-                  half_type(scale.scalar_type()), s.tiles, s.nw, s.kw, s.kz, s.kz > 1 ? part.data_ptr() : nullptr, w.stream),
+                  half_type(scale.scalar_type()), s.tiles, s.nw, s.kw, s.kz, s.kz > 1 ? part.data_ptr() : nullptr, s.kz > 1 ? part.numel() : 0, w.stream),
            "dlamd_int4_linear");
   return THPVariable_Wrap(std::move(y));
 }

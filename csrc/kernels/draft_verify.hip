@@ -8,6 +8,7 @@
 // Whether a token is taken or which v is hit is a comparison at a border, so probabilities are multiplied, subtracted and
 // summed in 64 bits: a product of two 32-bit numbers is exact there, and a sum of 2^17 of them is off by 2^-36 at most.
 #include "common.h"
+#include "decode_abi.h"
 
 typedef _Float16 f16_t;
 
@@ -366,11 +367,11 @@ static void launch_verify(const VerifyArgs& a, hipStream_t stream) {
 // sums: [B][pieces][2] doubles where pieces > 1.
 extern "C" int dlamd_verify_draft(const void* draft, long long d_bs, const void* p, long long p_bs, long long p_ns,
                                   const void* q, long long q_bs, long long q_ns, const void* u, long long u_bs,
-                                  const void* counts, void* tokens, void* accepted, void* sums, int pieces, int B, int n,
+                                  const void* counts, void* tokens, void* accepted, void* sums, long long sums_doubles, int pieces, int B, int n,
                                   int V, int pad, int dtype, hipStream_t stream) {
   if (B <= 0) return 0;
   if (n < 0 || n > 63 || V <= 0 || V >= 0x40000000) return -1;
-  if (pieces < 1 || pieces > 64 || (pieces > 1 && (B > 65535 || !sums || ((uintptr_t)sums & 7)))) return -3;
+  if (pieces < 1 || pieces > 64 || (pieces > 1 && (B > 65535 || !sums || ((uintptr_t)sums & 7) || sums_doubles < 2LL * B * pieces))) return -3;
   VerifyArgs a{(const int*)draft, p, q, (const float*)u, (const int*)counts, (int*)tokens, (int*)accepted, d_bs, p_bs, p_ns,
                q_bs, q_ns, u_bs, (double*)sums, B, n, V, pad, pieces};
   if (dtype == 0) launch_verify<bf16_t>(a, stream);

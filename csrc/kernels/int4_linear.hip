@@ -16,6 +16,7 @@
 // The waves of a workgroup share R tiles of 16 outputs and split K between them, 128 features at a time; their sums meet in
 // LDS.  The next step's loads are in flight while a step is computed.
 #include "common.h"
+#include "decode_abi.h"
 
 typedef _Float16 f16_t;
 
@@ -319,7 +320,7 @@ static void launch4_r(const Int4Args& a, int R, int CT, int G, int nw, hipStream
 extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, const void* scale, const void* zero,
                                  const void* bias, const void* res, long long res_rs, void* y, int M, int N, int K, int G,
                                  int act, int dtype, int sdtype, int tiles, int nw, int kw, int kz, void* part,
-                                 hipStream_t stream) {
+                                 long long part_floats, hipStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || (G != 32 && G != 64 && G != 128) || K % G != 0 || N > 0x7ffffff0) return -1;
   if (x_rs < 0 || x_rs >= (1 << 24) || K >= (1 << 24)) return -9;   // a workgroup's 32 rows of x: 31-bit offsets
@@ -329,7 +330,7 @@ extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, c
   const int CT = M <= 16 ? 1 : 2;
   if ((M + 16 * CT - 1) / (16 * CT) > 65535) return -5;
   if ((tiles != 1 && tiles != 2 && tiles != 4) || nw < 1 || kw < 1 || nw * kw > 8 || nw * kw * tiles * CT > 64) return -6;
-  if (kz < 1 || kz > 64 || (kz > 1 && (!part || ((uintptr_t)part & 15)))) return -7;
+  if (kz < 1 || kz > 64 || (kz > 1 && (!part || ((uintptr_t)part & 15) || part_floats < (long long)kz * M * ((N + 15) / 16 * 16)))) return -7;
   if ((long long)M * ((N + 15) / 16 * 4) > 0x7fffffffLL * 256) return -8;
   Int4Args a{x, (const uint32_t*)w, scale, (const uint8_t*)zero, (const float*)bias, res, y, x_rs, res_rs, (float*)part,
              M, N, K, act, kw, kz, zero ? 1 : 0};

@@ -8,6 +8,7 @@
 // Pure data movement (every byte is read once and written once), so the kernel is a flat list of 16-byte units: a unit
 // is one 8-dimension chunk, or, for half-split pairs, the two chunks that turn into each other.
 #include "common.h"
+#include "decode_abi.h"
 
 typedef _Float16 f16_t;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

@@ -6,8 +6,8 @@
 // are never used in arithmetic, whatever they hold.  A row without visible positions is 0, its log-sum-exp -inf.
 //
 // The cost is reading the cache once, so everything serves loads in flight:
-//   * The n new tokens x (heads / kv_heads) query heads that read one key head are the rows of ONE problem (16, 32 or 64
-//     per workgroup): a key is fetched once for all of them and the products run on matrix instructions, padded to 16.
+//   * The n new tokens x (heads / kv_heads) query heads that read one key head are the rows of ONE problem (up to 48 per
+//     workgroup): a key is fetched once for all of them and the products run on matrix instructions, padded to 16.
 //   * A wave takes tiles of 32 keys by itself, straight from memory into the operand registers, the next tile's loads in
 //     flight while it computes; no LDS, no barrier until the four waves of a workgroup join their (m, l, o).
 //   * S^T = K Q^T: A = K (a lane holds 8 dimensions of one key, as they lie in memory), so a lane's accumulators are 4 keys
@@ -17,11 +17,12 @@
 //     then holds dimension (D / 16) r + i in row r, which leaves a lane with D / 4 consecutive dimensions of one query.
 //   * P goes into the products as two 16-bit halves, hi + lo: one rounding to 16 bits would cost as much accuracy as the
 //     result's own rounding, and the second product hides behind the loads.
-//   * Long caches are cut into parts of as many tiles (of 128 or 64 keys) as give every compute unit its share.  The size of a
+//   * Long caches are cut into parts of as many tiles (of 128 keys) as give every compute unit its share.  The size of a
 //     part is computed on the device from the lengths of the whole batch, so neither one long sequence nor a batch of very
 //     different lengths leaves compute units idle, and a captured call adapts while lengths grow.  A part is written as
 //     (m, l, o) in 32 bits and a second kernel joins the parts.  Short caches (and many of them) take one workgroup each.
 #include "common.h"
+#include "decode_abi.h"
 
 typedef _Float16 f16_t;
 
@@ -42,19 +43,33 @@ struct PagedAttArgs {
   int groups, rows, share, least;                            // row groups per (b, kv head), rows per group; workgroups to deal
                                                              // tiles out to (0: one for each problem), least tiles of a part
   uint32_t page_magic;                                       // ceil(2^32 / (page / 16))
-  float scale2;                                              // scale * log2(e)
+  float scale2;                                              // |scale| log2(e), above 0
+  uint32_t flip;                                             // sign bits to turn in q where the scale is negative
 };
 
 #define ROW_NONE (-3.4028234e38f)                            // running maximum of nothing: finite, so differences stay numbers
 #define LN2 0.6931471805599453f
 
+// mul: a 16x16x32 product; split: two weights as 16-bit halves hi + lo (hi may be rounded either way, lo makes up for it).
 template <typename T> struct Mat;
 template <> struct Mat<bf16_t> {
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 x2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const x2 h = {(__bf16)a, (__bf16)b};
+    hi = __builtin_bit_cast(uint32_t, h);
+    const x2 l = {(__bf16)(a - __builtin_bit_cast(float, hi << 16)), (__bf16)(b - __builtin_bit_cast(float, hi & 0xffff0000u))};
+    lo = __builtin_bit_cast(uint32_t, l);
+  }
   static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mat<f16_t> {
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+  }
   static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
@@ -73,11 +88,12 @@ struct Place {
   bool ok[2];                                                // the half's page exists and some row sees it
 };
 
-// Page of the 16 keys at `key` (beyond the limit: none).  Uniform over the wave: the entry comes by a scalar load.
-__device__ __forceinline__ int page_of(const PagedAttArgs& p, const_i32 row, int key, int limit) {
+// Page of the 16 keys at `key`, whether or not they lie below the limit (behind the table: its last entry).  Uniform over the
+// wave: the entry comes by a scalar load, without a branch.
+__device__ __forceinline__ int page_of(const PagedAttArgs& p, const_i32 row, int key) {
   const int unit = key >> 4;
   const int pi = p.page_magic ? (int)__umulhi((uint32_t)unit, p.page_magic) : unit;
-  return key < limit ? row[pi] : -1;
+  return row[min(pi, p.width - 1)];
 }
 
 // Rows that no one sees are not skipped but replaced by rows that are there (the limit's last one, or zeros for a missing
@@ -90,7 +106,7 @@ __device__ __forceinline__ void find_tile(Place& t, const PagedAttArgs& p, globa
     const int unit = key >> 4;
     const int pi = p.page_magic ? (int)__umulhi((uint32_t)unit, p.page_magic) : unit;
     const int slot = key - pi * p.page;
-    t.ok[h] = pid >= 0 && pid < p.pages;
+    t.ok[h] = key < limit && pid >= 0 && pid < p.pages;
     t.k[h] = t.ok[h] ? kh + pid * p.k_ps + slot * p.k_ss : (global_p)k_zero_row;
     t.v[h] = t.ok[h] ? vh + pid * p.v_ps + slot * p.v_ss : (global_p)k_zero_row;
     t.ks[h] = t.ok[h] ? p.k_ss : 0;
@@ -136,13 +152,13 @@ struct Rows {                                                // what a wave hold
   typename Mat<T>::x8 q[MT][D / 32];
 };
 
-// Scores of one tile (in units of log 2), -inf where a row does not see the key.
+// Scores of one tile before scaling, -inf where a row does not see the key.
 template <typename T, int D, int MT, bool TAIL>
 __device__ __forceinline__ void scores(f32x4 (&x)[MT][2], const Rows<T, D, MT>& w, const u32x4 (&k)[2][D / 32], const Place& t,
-                                       const PagedAttArgs& p, int k0, int g) {
+                                       int k0, int g) {
   typedef typename Mat<T>::x8 x8;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int seen = (t.ok[h] ? TAIL ? w.lim[mt] : 0x7fffffff : 0) - (k0 + 16 * h + 4 * g);
@@ -150,19 +166,21 @@ __device__ __forceinline__ void scores(f32x4 (&x)[MT][2], const Rows<T, D, MT>& 
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) s = Mat<T>::mul(__builtin_bit_cast(x8, k[h][c]), w.q[mt][c], s);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[mt][h][j] = (TAIL ? j < seen : t.ok[h]) ? s[j] * p.scale2 : -INFINITY;
+      for (int j = 0; j < 4; ++j) x[mt][h][j] = (TAIL ? j < seen : t.ok[h]) ? s[j] : -INFINITY;
     }
+  }
 }
 
-// Scores to weights, against the running maximum.
+// Scores to weights, against the running maximum (which is kept scaled, in units of log 2).
 template <typename T, int D, int MT>
 __device__ __forceinline__ void weights(typename Mat<T>::x8 (&hi)[MT], typename Mat<T>::x8 (&lo)[MT], Rows<T, D, MT>& w,
-                                        const f32x4 (&x)[MT][2]) {
+                                        const f32x4 (&x)[MT][2], float scale2) {
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    float top = ROW_NONE;
+    float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(x[mt][0][j], x[mt][1][j]));
+    top *= scale2;
     if (__any(top > w.m[mt])) {                              // rare once the largest scores have been seen
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -176,16 +194,20 @@ __device__ __forceinline__ void weights(typename Mat<T>::x8 (&hi)[MT], typename 
         for (int j = 0; j < 4; ++j) w.o[mt][i][j] *= a;
     }
     float sum = 0.f;
+    u32x4 h4, l4;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = __builtin_amdgcn_exp2f(x[mt][h][j] - w.m[mt]);
-        sum += e;
-        const T eh = (T)e;
-        hi[mt][4 * h + j] = eh;
-        lo[mt][4 * h + j] = (T)(e - (float)eh);
-      }
+    for (int c = 0; c < 4; ++c) {
+      const int h = c >> 1, j = 2 * (c & 1);
+      const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[mt][h][j], scale2, -w.m[mt]));
+      const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[mt][h][j + 1], scale2, -w.m[mt]));
+      sum += e0 + e1;
+      uint32_t a, b;
+      Mat<T>::split(e0, e1, a, b);
+      h4[c] = a;
+      l4[c] = b;
+    }
+    hi[mt] = __builtin_bit_cast(typename Mat<T>::x8, h4);
+    lo[mt] = __builtin_bit_cast(typename Mat<T>::x8, l4);
     w.l[mt] += sum;                                          // this lane's keys; the four lane groups join at the end
   }
 }
@@ -223,7 +245,7 @@ __device__ __forceinline__ void add_values(Rows<T, D, MT>& w, uint32_t (&v)[8][D
       a[c] = __builtin_amdgcn_perm(v[2 * c + 1][i >> 1], v[2 * c][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      w.o[mt][i] = Mat<T>::mul(__builtin_bit_cast(x8, a), hi[mt], w.o[mt][i]);
+        w.o[mt][i] = Mat<T>::mul(__builtin_bit_cast(x8, a), hi[mt], w.o[mt][i]);
       w.o[mt][i] = Mat<T>::mul(__builtin_bit_cast(x8, a), lo[mt], w.o[mt][i]);
     }
   }
@@ -261,7 +283,7 @@ __device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedA
 #pragma unroll
           for (int j = 0; j < 8; ++j) x += (float)a[j] * (float)c[j];
         }
-        const float e = __builtin_amdgcn_exp2f(x * p.scale2 - w.m[mt]);
+        const float e = __builtin_amdgcn_exp2f((p.flip ? -x : x) * p.scale2 - w.m[mt]);
 #pragma unroll
         for (int d = 0; d < D / 4; d += 8) {                 // the lane's sums: dimensions D / 4 g .. of its query
           const x8 v = *reinterpret_cast<const x8*>(vr + d);
@@ -273,10 +295,10 @@ __device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedA
   }
 }
 
-// Tiles of sequence b (at least one: an empty sequence's rows are written, too).
+// Tiles of a sequence that keeps so many tokens (at least one: an empty sequence's rows are written, too).
 template <int TK>
-__device__ __forceinline__ int tiles_of(const PagedAttArgs& p, int b) {
-  const int kept = ((const_i32)p.lens)[b], cap = p.width * p.page;
+__device__ __forceinline__ int tiles_of(const PagedAttArgs& p, int kept) {
+  const int cap = p.width * p.page;
   const int limit = kept < 0 || p.pages == 0 ? 0 : min(min(kept, cap) + (p.causal ? p.n : 0), cap);
   return max(1, (limit + TK - 1) / TK);
 }
@@ -298,35 +320,39 @@ __device__ __forceinline__ int wave_scan_i32(int v) {
 template <int TK>
 __device__ __forceinline__ int tiles_each(const PagedAttArgs& p, int H, int lane, int mine) {
   int sum = mine;                                            // tiles of sequence `lane`
-  for (int b = lane + 64; b < p.B; b += 64) sum += tiles_of<TK>(p, b);
+  for (int b = lane + 64; b < p.B; b += 64) sum += tiles_of<TK>(p, p.lens[b]);
   const int total = __builtin_amdgcn_readlane(wave_scan_i32(sum), 63) * H;
   return max(p.least, (total + p.share - 1) / p.share);
 }
 
-template <typename T, int D, int MT, int RW>
-__global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(const PagedAttArgs p) {
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_attention_kernel(const PagedAttArgs p) {
   typedef typename Mat<T>::x8 x8;
-  constexpr int KW = 4 / RW, TK = 32 * KW;                   // RW waves over rows, KW over keys
+  constexpr int TK = 128;                                    // keys of a tile: 32 for each wave
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ float s_o[4][16][D + 4];                        // + 4: lanes of one group write 16 rows at once
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4, rw = RW == 1 ? 0 : wave / KW, kw = RW == 1 ? wave : wave % KW;
+  const int r = lane & 15, g = lane >> 4;
   const int G = p.Hq / p.Hkv, R = p.n * G, H = p.Hkv * p.groups;
   const int cap = p.width * p.page, me = blockIdx.x;
 
   // which problem and which of its tiles
-  int b, head, tile = 0, tiles = 0x7fffffff;
+  int b, head, kept, tile = 0, tiles = 0x7fffffff;
   bool whole = true;
   if (p.share == 0) {
     b = me / H;
     head = me - b * H;
+    b = __builtin_amdgcn_readfirstlane(b);
+    kept = ((const_i32)p.lens)[b];
   } else {
-    const int t0 = lane < p.B ? tiles_of<TK>(p, lane) : 0;
+    int mine = lane < p.B ? p.lens[lane] : 0;
+    const int t0 = lane < p.B ? tiles_of<TK>(p, mine) : 0;
     const int each = tiles_each<TK>(p, H, lane, t0);
     int begin = 0, src = -1, upto = 0, parts = 0;
     b = 0;
     for (; b < p.B; b += 64) {                               // the sequence of part `me`, 64 of them at a time
-      const int t = b == 0 ? t0 : b + lane < p.B ? tiles_of<TK>(p, b + lane) : 0;
+      if (b) mine = b + lane < p.B ? p.lens[b + lane] : 0;
+      const int t = b == 0 ? t0 : b + lane < p.B ? tiles_of<TK>(p, mine) : 0;
       parts = (t + each - 1) / each;
       upto = begin + wave_scan_i32(parts * H);
       const unsigned long long past = __ballot(upto > me);
@@ -338,6 +364,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(c
     }
     if (src < 0) return;                                     // fewer parts than workgroups
     b += src;
+    kept = __builtin_amdgcn_readlane(mine, src);
     parts = __builtin_amdgcn_readlane(parts, src);
     const int in = me - (__builtin_amdgcn_readlane(upto, src) - parts * H);
     head = in / parts;
@@ -349,37 +376,41 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(c
   head = __builtin_amdgcn_readfirstlane(head);
   tile = __builtin_amdgcn_readfirstlane(tile);
 
-  const int hk = head / p.groups, row0 = (head - hk * p.groups) * p.rows + rw * 16 * MT;
-  const int kept = ((const_i32)p.lens)[b];
-  const int base = kept < 0 || p.pages == 0 ? 0 : min(kept, cap), more = kept >= 0 && p.pages > 0 && p.causal;
-  // limits of the wave's first and last row
-  const int rl = min(row0 + 16 * MT, R) - 1;
-  const int limit_all = min(base + (more ? row0 / G + 1 : 0), cap);
-  const int limit = row0 < R ? (int)min((long long)min(base + (more ? rl / G + 1 : 0), cap), ((long long)tile + tiles) * TK) : 0;
-
+  // the first pages are asked for together with the length, not after it
+  const const_i32 row = (const_i32)p.table + b * p.t_bs;
+  const int kb = tile * TK;
+  int k0 = kb + 32 * wave;
+  const int first0 = page_of(p, row, k0), first1 = page_of(p, row, k0 + 16);
+  int pid0 = page_of(p, row, k0 + TK), pid1 = page_of(p, row, k0 + TK + 16);
+  const int hk = head / p.groups, row0 = (head - hk * p.groups) * p.rows;
   Rows<T, D, MT> w;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int row = row0 + 16 * mt + r;
-    const int i = row / G, h = hk * G + row - i * G;
-    w.lim[mt] = row < R ? min(min(base + (more ? i + 1 : 0), cap), limit) : 0;
-    w.m[mt] = ROW_NONE;
-    w.l[mt] = 0.f;
+    const int row = row0 + 16 * mt + r, i = row / G, h = hk * G + row - i * G;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       u32x4 t = {0u, 0u, 0u, 0u};
       if (row < R) t = *reinterpret_cast<const u32x4*>((const T*)p.q + b * p.q_bs + i * p.q_ns + h * p.q_hs + 32 * c + 8 * g);
-      w.q[mt][c] = __builtin_bit_cast(x8, t);
+      w.q[mt][c] = __builtin_bit_cast(x8, t ^ p.flip);
     }
+  }
+  const int base = kept < 0 || p.pages == 0 ? 0 : min(kept, cap), more = kept >= 0 && p.pages > 0 && p.causal;
+  // limits of the first and last row
+  const int rl = min(row0 + 16 * MT, R) - 1;
+  const int limit_all = min(base + (more ? row0 / G + 1 : 0), cap);
+  const int limit = (int)min((long long)min(base + (more ? rl / G + 1 : 0), cap), ((long long)tile + tiles) * TK);
 #pragma unroll
-    for (int i2 = 0; i2 < D / 16; ++i2) w.o[mt][i2] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = row0 + 16 * mt + r;
+    w.lim[mt] = row < R ? min(min(base + (more ? row / G + 1 : 0), cap), limit) : 0;
+    w.m[mt] = ROW_NONE;
+    w.l[mt] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) w.o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   // The next tile's keys are fetched into the registers of this one's as soon as the scores have been taken, its values
   // after the products: at any time a wave has most of a tile in flight, and three waves fit a SIMD.
-  const const_i32 row = (const_i32)p.table + b * p.t_bs;
   const global_p kh = (global_p)p.kp + (long long)hk * p.k_hs, vh = (global_p)p.vp + (long long)hk * p.v_hs;
-  const int kb = tile * TK;
-  int k0 = kb + 32 * kw;
   bool odd = false;
   if (k0 < limit) {
     u32x4 k[2][D / 32];
@@ -387,27 +418,26 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(c
     Place pl;
     x8 hi[MT], lo[MT];
     f32x4 x[MT][2];
-    find_tile(pl, p, kh, vh, page_of(p, row, k0, limit), page_of(p, row, k0 + 16, limit), k0, limit);
+    find_tile(pl, p, kh, vh, first0, first1, k0, limit);
     load_k<D, true>(k, pl, r, g);
     load_v<D, true>(v, pl, r, g);
-    int pid0 = page_of(p, row, k0 + TK, limit), pid1 = page_of(p, row, k0 + TK + 16, limit);
-    // All tiles but a wave's last end more than 32 keys before the wave's limit, and its first row's limit is at most 31
-    // keys before that: every row sees them.  No load here has a condition: where a path with loads meets one without, the
-    // compiler can only wait for all of them.
+    // All tiles but a wave's last end more than 96 keys before the limit, and the first row's limit is at most 63 keys before
+    // that: every row sees them.  No load here has a condition: where a path with loads meets one without, the compiler can
+    // only wait for all of them.
     for (; k0 + TK < limit; k0 += TK) {
-      scores<T, D, MT, false>(x, w, k, pl, p, k0, g);
+      scores<T, D, MT, false>(x, w, k, pl, k0, g);
       Place next;
       find_tile(next, p, kh, vh, pid0, pid1, k0 + TK, limit);
       load_k<D, true>(k, next, r, g);
-      pid0 = page_of(p, row, k0 + 2 * TK, limit);
-      pid1 = page_of(p, row, k0 + 2 * TK + 16, limit);
-      weights<T, D, MT>(hi, lo, w, x);
+      pid0 = page_of(p, row, k0 + 2 * TK);
+      pid1 = page_of(p, row, k0 + 2 * TK + 16);
+      weights<T, D, MT>(hi, lo, w, x, p.scale2);
       add_values<T, D, MT, false>(w, v, hi, lo, pl, k0, limit_all, limit, g, odd);
       load_v<D, true>(v, next, r, g);
       pl = next;
     }
-    scores<T, D, MT, true>(x, w, k, pl, p, k0, g);
-    weights<T, D, MT>(hi, lo, w, x);
+    scores<T, D, MT, true>(x, w, k, pl, k0, g);
+    weights<T, D, MT>(hi, lo, w, x, p.scale2);
     add_values<T, D, MT, true>(w, v, hi, lo, pl, k0, limit_all, limit, g, odd);
   }
 #pragma unroll
@@ -416,9 +446,9 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(c
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) odd |= w.o[mt][i][j] != w.o[mt][i][j];
-  if (__any(odd)) add_values_again<T, D, MT, TK>(w, p, row, b, hk, row0, R, G, kb + 32 * kw, limit, r, g);
+  if (__any(odd)) add_values_again<T, D, MT, TK>(w, p, row, b, hk, row0, R, G, kb + 32 * wave, limit, r, g);
   float* part = p.part + (long long)me * p.rows * (D + 4);
-  // join the waves over keys, 16 rows of each wave over rows at a time
+  // join the four waves, 16 rows at a time
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float l = w.l[mt];
@@ -438,26 +468,21 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(c
       }
     __syncthreads();
     // a thread: D / 16 dimensions of a row
+    const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16), in = 16 * mt + rr, row = row0 + in;
+    if (in < p.rows && row < R) {
+      const float m = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]), fmaxf(s_m[2][rr], s_m[3][rr]));
+      float f[4], sum = 0.f;
 #pragma unroll
-    for (int q = 0; q < RW; ++q) {
-      const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
-      const int in = (q * MT + mt) * 16 + rr, row = (head - hk * p.groups) * p.rows + in;
-      if (in >= p.rows || row >= R) continue;
-      float m = s_m[q * KW][rr];
-#pragma unroll
-      for (int x = 1; x < KW; ++x) m = fmaxf(m, s_m[q * KW + x][rr]);
-      float f[KW], sum = 0.f;
-#pragma unroll
-      for (int x = 0; x < KW; ++x) {
-        f[x] = __builtin_amdgcn_exp2f(s_m[q * KW + x][rr] - m);
-        sum += f[x] * s_l[q * KW + x][rr];
+      for (int x = 0; x < 4; ++x) {
+        f[x] = __builtin_amdgcn_exp2f(s_m[x][rr] - m);
+        sum += f[x] * s_l[x][rr];
       }
       float o[D / 16];
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         o[d] = 0.f;
 #pragma unroll
-        for (int x = 0; x < KW; ++x) o[d] += f[x] * s_o[q * KW + x][rr][d0 + d];
+        for (int x = 0; x < 4; ++x) o[d] += f[x] * s_o[x][rr][d0 + d];
       }
       if (whole) {
         const int i = row / G, h = hk * G + row - i * G;
@@ -484,8 +509,9 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void paged_attention_kernel(c
 }
 
 // One workgroup per row: joins the parts of its sequence.
-template <typename T, int D, int TK>
+template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttArgs p) {
+  constexpr int TK = 128;
   constexpr int TD = D / 4, SL = 256 / TD;                   // threads per part (4 dimensions each), parts side by side
   __shared__ float s_o[SL][D];
   __shared__ float s_l[SL], s_m[SL];
@@ -494,12 +520,13 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
   const int G = p.Hq / p.Hkv, H = p.Hkv * p.groups, hk = h / G;
   const int row = i * G + h - hk * G, group = row / p.rows, in = row - group * p.rows;
   const int lane = threadIdx.x & 63;
-  const int t0 = lane < p.B ? tiles_of<TK>(p, lane) : 0;
+  const int own = ((const_i32)p.lens)[b];
+  const int t0 = lane < p.B ? tiles_of<TK>(p, p.lens[lane]) : 0;
   const int each = tiles_each<TK>(p, H, lane, t0);
-  const int parts = (tiles_of<TK>(p, b) + each - 1) / each;
+  const int parts = (tiles_of<TK>(p, own) + each - 1) / each;
   if (parts == 1) return;                                    // written already
   int before = 0;                                            // parts of the sequences before this one
-  for (int x = lane; x < b; x += 64) before += ((x == lane ? t0 : tiles_of<TK>(p, x)) + each - 1) / each;
+  for (int x = lane; x < b; x += 64) before += ((x == lane ? t0 : tiles_of<TK>(p, p.lens[x])) + each - 1) / each;
   const int lo = __builtin_amdgcn_readlane(wave_scan_i32(before), 63) * H + (hk * p.groups + group) * parts;
   const int d = (threadIdx.x % TD) * 4, sl = threadIdx.x / TD;
   const float* src = p.part + (long long)in * (D + 4);
@@ -537,27 +564,28 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
   }
 }
 
-template <typename T, int D, int MT, int RW>
+template <typename T, int D, int MT>
 static void launch(const PagedAttArgs& a, hipStream_t stream) {
   const unsigned grid = a.share + a.B * a.Hkv * a.groups;
-  hipLaunchKernelGGL((paged_attention_kernel<T, D, MT, RW>), dim3(grid), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((paged_attention_kernel<T, D, MT>), dim3(grid), dim3(256), 0, stream, a);
   if (a.share)
-    hipLaunchKernelGGL((paged_attention_join_kernel<T, D, 128 / RW>), dim3((unsigned)(a.B * a.n * a.Hq)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((paged_attention_join_kernel<T, D>), dim3((unsigned)(a.B * a.n * a.Hq)), dim3(256), 0, stream, a);
 }
 template <typename T, int D>
-static void launch_rows(const PagedAttArgs& a, int R, hipStream_t stream) {
-  if (R <= 16) launch<T, D, 1, 1>(a, stream);
-  else if (R <= 32) launch<T, D, 2, 1>(a, stream);
-  else launch<T, D, 2, 2>(a, stream);
+static void launch_rows(const PagedAttArgs& a, int rows, hipStream_t stream) {
+  if (rows <= 16) launch<T, D, 1>(a, stream);
+  else if (rows <= 32) launch<T, D, 2>(a, stream);
+  else launch<T, D, 3>(a, stream);
 }
 
 // q: [B, n, Hq, D] (strides given), o: [B, n, Hq, D] contiguous, lse: [B, n, Hq] or null.  dtype: 0 bf16, 1 fp16.
 // share: 0 (a workgroup per sequence, key head and group of rows) or workgroups to deal all tiles out to, in parts of at least
-// `least` tiles; part: [share + problems][rows][D + 4] floats where share > 0, rows = min(n Hq / Hkv, 64).
+// `least` tiles; part: [share + problems][rows of a problem][D + 4] floats where share > 0.
 extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_ns, long long q_hs, const void* kp,
                                      long long kp_ps, long long kp_ss, long long kp_hs, const void* vp, long long vp_ps,
                                      long long vp_ss, long long vp_hs, const void* table, long long t_bs,
-                                     const void* lens, void* o, void* lse, void* part, int share, int least, int B, int n,
+                                     const void* lens, void* o, void* lse, void* part, long long part_floats,
+                                     int share, int least, int B, int n,
                                      int Hq, int Hkv, int D, int page, int width, int pages, int causal, float scale,
                                      int dtype, hipStream_t stream) {
   if (B <= 0 || n <= 0 || Hq <= 0) return 0;
@@ -575,18 +603,27 @@ extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_
   if (dtype != 0 && dtype != 1) return -6;
   if (share < 0 || share > (1 << 20) || (share > 0 && (least < 1 || !part || ((uintptr_t)part & 15)))) return -7;
   if ((long long)n * Hq > 0x7fffffffLL || (long long)B * n * Hq > 0x7fffffffLL) return -9;
-  // rows of one problem: up to 16 (one tile of queries), 32 (two), 64 (two waves with two)
-  const int R = n * (Hq / Hkv), rows = R < 64 ? R : 64, groups = (R + 63) / 64;
+  // Rows of one problem, in tiles of 16.  Up to 48 share a key's fetch (12 ragged caches, 40 rows: 26 us; as two groups that
+  // fetch it twice 31); beyond, groups of up to 32 (64 rows in one wave: 30 us for 2 x 16384 keys, in two groups 26.5: the
+  // registers of more rows leave one workgroup per compute unit).
+  const int R = n * (Hq / Hkv), groups = R <= 48 ? 1 : (R + 31) / 32, rows = (R + groups - 1) / groups;
+  if (share > 0 && part_floats < ((long long)share + (long long)B * Hkv * groups) * rows * (D + 4)) return -12;
   // problems, parts and tiles are counted in 32 bits
   if (((long long)B * Hkv * groups + share) * ((long long)width * page / 64 + 2) > 0x7fffffffLL) return -10;
+  if (width == 0) {                                          // no table to read: one entry of anything, and no pages
+    table = lens;
+    t_bs = 0;
+    width = 1;
+    pages = 0;
+  }
   const uint32_t units = (uint32_t)(page / 16);
   const uint32_t magic = units == 1 ? 0u : (uint32_t)((0x100000000ULL + units - 1) / units);
   PagedAttArgs a{q, kp, vp, o, (float*)lse, (float*)part, (const int*)table, (const int*)lens, q_bs, q_ns, q_hs,
                  kp_ps * 2, vp_ps * 2, t_bs, (int)sl[0], (int)sl[2], (int)sl[1], (int)sl[3], B, n, Hq, Hkv, page, width, pages, causal,
-                 groups, rows, share, least, magic, scale * 1.4426950408889634f};
-  if (dtype == 0 && D == 64) launch_rows<bf16_t, 64>(a, R, stream);
-  if (dtype == 0 && D == 128) launch_rows<bf16_t, 128>(a, R, stream);
-  if (dtype == 1 && D == 64) launch_rows<f16_t, 64>(a, R, stream);
-  if (dtype == 1 && D == 128) launch_rows<f16_t, 128>(a, R, stream);
+                 groups, rows, share, least, magic, fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f), scale < 0.f ? 0x80008000u : 0u};
+  if (dtype == 0 && D == 64) launch_rows<bf16_t, 64>(a, rows, stream);
+  if (dtype == 0 && D == 128) launch_rows<bf16_t, 128>(a, rows, stream);
+  if (dtype == 1 && D == 64) launch_rows<f16_t, 64>(a, rows, stream);
+  if (dtype == 1 && D == 128) launch_rows<f16_t, 128>(a, rows, stream);
   return DLAMD_CHECK_LAUNCH();
 }

@@ -167,7 +167,7 @@ def build_bind(force: bool = False, verbose: bool = False) -> Path:
     srcs = sorted((CSRC / "bind").glob("*.cpp"))
     out = LIB_DIR / "dlamd_bind.so"
     flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    digest = _sha(srcs, " ".join(flags) + torch.__version__ + sys.version)
+    digest = _sha([*srcs, CSRC / "kernels" / "decode_abi.h"], " ".join(flags) + torch.__version__ + sys.version)
     if not force and _up_to_date("bind", digest, out):
         return out
     LIB_DIR.mkdir(parents=True, exist_ok=True)

@@ -311,6 +311,17 @@ def test_attention_kernel_with_peaked_scores():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.1, 0.02, 1.5])
+def test_attention_kernel_with_other_scales(scale):
+    c = att_case(8, [90, 300], 2, 16, 4, 2, 64, torch.bfloat16, True, qscale=0.3)
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o, lse = P.paged_attention(**d, scale=scale, return_lse=True)
+    ref, ref_lse = P.paged_attention_reference(**c, scale=scale, dtype=torch.float64)
+    assert bool(((o.cpu().double() - ref).abs() <= att_tolerance(c, ref)).all())
+    assert bool(((lse.cpu().double() - ref_lse).abs() <= 2.0 ** -24 * 130 * 64).all())
+
+
+@pytest.mark.gpu
 def test_attention_kernel_with_infinite_and_nan_keys_in_sight():
     """A visible key whose score is -inf weighs nothing; a NaN in a visible value reaches its own row only."""
     c = att_case(6, [50, 50], 1, 16, 2, 2, 64, torch.bfloat16, True)
