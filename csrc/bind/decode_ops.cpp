@@ -197,12 +197,13 @@ PyObject* attention(PyObject* const* a) {
 }
 
 // ------------------------------------------------------------------------------------------ verification
-// Workgroups that share a row.  Up to 8192 tokens one holds the row in registers (8 x 4000: 5.8 us, 8.5 in pieces); a large
-// batch keeps the card busy by itself (192 x 50265: 24 us, 21.6 in 32 pieces with a second launch); 1 x 50265: 8.2 us in 48
-// pieces, 17.6 in one.
-int64_t pieces_of(int64_t B, int64_t V) {
-  if (V <= 8192 || B >= 128) return 1;
-  return B < 32 ? std::min<int64_t>(48, (V + 511) / 512) : std::min<int64_t>(32, (V + 2047) / 2048);
+// Workgroups that share a sequence's row of `bytes` (target's and proposal's).  Up to 8192 tokens one holds it in registers
+// (8 x 4000: 5.7 us, 8.7 in pieces).  128 short rows keep the card busy by themselves (256 x 32000 bf16: 15.3 us, in pieces
+// 16.7), long ones are dealt out more evenly in pieces (192 x 50265 fp32: 21.6 us in 32, 23.3 in one; 512 x 50265: 38.8 and
+// 45.9).  Fewer rows than compute units want more pieces (1 x 50265: 8.3 us in 48, 17.6 in one).
+int64_t pieces_of(int64_t B, int64_t V, int64_t bytes) {
+  if (V <= 8192 || (B >= 128 && bytes < 256 << 10) || B > 65535) return 1;
+  return B < 32 ? std::min<int64_t>(48, (V + 511) / 512) : std::min<int64_t>(32, (V + 1535) / 1536);
 }
 
 // (draft, target, u, proposal, counts, pad, pieces or None, stream) -> (tokens, accepted)
@@ -229,9 +230,9 @@ PyObject* verify(PyObject* const* a) {
   need(pad >= -0x80000000LL && pad <= 0x7fffffffLL, "pad is an int32");
   const Where w(draft, a[7]);
   at::Tensor tokens = at::empty({B, n + 1}, draft.options()), accepted = at::empty({B}, draft.options()), sums;
-  const int64_t pieces = a[6] == Py_None ? pieces_of(B, V) : number(a[6]);
-  if (pieces > 1) sums = at::empty({B, pieces, 2}, draft.options().dtype(at::kDouble));
   const bool with_q = proposal && n > 0;
+  const int64_t pieces = a[6] == Py_None ? pieces_of(B, V, V * target.element_size() * (with_q ? 2 : 1)) : number(a[6]);
+  if (pieces > 1) sums = at::empty({B, pieces, 2}, draft.options().dtype(at::kDouble));
   launched(k_verify(draft.data_ptr(), draft.stride(0), target.data_ptr(), target.stride(0), target.stride(1), with_q ? proposal.ptr() : nullptr,
                     with_q ? proposal->stride(0) : 0, with_q ? proposal->stride(1) : 0, u.data_ptr(), u.stride(0), counts.ptr(),
                     tokens.data_ptr(), accepted.data_ptr(), pieces > 1 ? sums.data_ptr() : nullptr, pieces > 1 ? sums.numel() : 0, as_int(pieces), as_int(B), as_int(n),
@@ -326,12 +327,12 @@ PyObject* init(PyObject* const* a) {
   k_error = a[4];
   Py_RETURN_NONE;
 }
-// (problems, rows, bound, D), (B, V), (M, N, K): the rules above, for tests
+// (problems, rows, bound, D), (B, V) of fp32 rows with a proposal, (M, N, K): the rules above, for tests
 PyObject* rule_deal(PyObject* const* a) {
   const Deal d = deal_out(number(a[0]), number(a[1]), number(a[2]), number(a[3]));
   return Py_BuildValue("(LL)", (ll)d.share, (ll)d.least);
 }
-PyObject* rule_pieces(PyObject* const* a) { return PyLong_FromLongLong(pieces_of(number(a[0]), number(a[1]))); }
+PyObject* rule_pieces(PyObject* const* a) { return PyLong_FromLongLong(pieces_of(number(a[0]), number(a[1]), number(a[1]) * 8)); }
 PyObject* rule_shape(PyObject* const* a) {
   const Shape s = shape_of(number(a[0]), number(a[1]), number(a[2]));
   return Py_BuildValue("(iiii)", s.tiles, s.nw, s.kw, s.kz);

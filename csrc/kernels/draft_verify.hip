@@ -333,14 +333,15 @@ __global__ __launch_bounds__(256) void verify_find_kernel(const VerifyArgs a) {
     total = lane_f64(upto, 63);
   }
   const double x = border(a, b, total);
-  const unsigned long long past = __ballot(rest > 0.0 && (upto > x || (x >= total && upto == total)));
+  // sums of lanes are associated differently, so an upto may lie a rounding beyond the total, or under the one before it
+  const unsigned long long past = __ballot(rest > 0.0 && upto > x), any = __ballot(rest > 0.0);
   if (threadIdx.x == 0) {
     s_hit[0] = 0x7fffffff;
     s_hit[1] = -1;                                           // a row without any weight: token 0
   }
-  if (past && total > 0.0 && total < INFINITY) {             // the same for every thread of the workgroup
-    const int at = __ffsll(past) - 1;
-    const double before = at ? lane_f64(upto, at - 1) : 0.0;
+  if (any && total > 0.0 && total < INFINITY) {              // the same for every thread of the workgroup
+    const int at = past ? __ffsll(past) - 1 : 63 - __clzll(any);
+    const double before = at ? fmin(lane_f64(upto, at - 1), x) : 0.0;
     const int piece = (a.V + a.pieces - 1) / a.pieces, p0 = at * piece, p1 = min(p0 + piece, a.V);
     find_in_piece<T, 4>(r, p0, p1, all, before, x, lane, wave, s_w, s_hit);
   }
