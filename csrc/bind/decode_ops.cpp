@@ -247,11 +247,28 @@ PyObject* verify(PyObject* const* a) {
 struct Shape {
   int tiles, nw, kw, kz;                                     // tiles of 16 outputs per wave, waves over outputs and K, parts of K
 };
+
+// The share of the 256 compute units that work while `groups` equal workgroups run, and what a further part of K costs
+// besides (its sums are written and read again).
+double fill(int64_t groups, int kz) { return (double)groups * kz / ((groups * kz + 255) / 256 * 256) - 0.06 * (kz - 1); }
+
+// Few outputs (N < 8192): one tile a wave and eight waves over K, the most waves the layer can have (1 x 4096 x 1024: 3.9 us,
+// with two tiles 4.4; 16 x 4096 x 4096: 7.7 and 8.1).  Many: two tiles share a wave's x where there is one tile of rows
+// (5 x 50265 x 1024: 9.7 us, with one 11.2), four where there are more (32 x 32000 x 8192: 47.5, with two 68).
+// Where a long K leaves the last round of workgroups mostly empty, parts of K even it out: 313 workgroups in four parts
+// (20 x 20000 x 8192, groups of 64) 40.3 us, in one 48.5; 128 in two (24 x 8192 x 28672) 41.3, in one 64.7; 250 in one
+// (32 x 32000 x 8192) 47.5, in two 53.3.
 Shape shape_of(int64_t M, int64_t N, int64_t K) {
   const int steps = (int)std::min<int64_t>((K + 127) / 128, 1 << 20);
   if (N < 8192) return {1, 1, std::min(8, steps), 1};
   if (M <= 16) return {2, 1, std::min(4, steps), 1};
-  return {4, 1, std::min(4, steps), N < 10000 && steps >= 64 ? 2 : 1};
+  int kz = 1;
+  if (steps >= 64) {
+    const int64_t groups = (N + 63) / 64 * ((M + 31) / 32);
+    for (int parts = 2; parts <= 4; ++parts)
+      if (fill(groups, parts) > fill(groups, kz)) kz = parts;
+  }
+  return {4, 1, std::min(4, steps), kz};
 }
 
 // (x, words, scale, zero, n, k, group, bias, act, res, shape or None, stream) -> y
@@ -267,11 +284,12 @@ PyObject* int4(PyObject* const* a) {
     need(res->dim() == dims && res->size(dims - 1) == N && res->sizes().slice(0, dims - 1) == x.sizes().slice(0, dims - 1) &&
              res->scalar_type() == x.scalar_type(),
          "res is [..., N] of x's type");
+  no_gradient({&x, bias.t, res.t});
   same_device(x.device(), {&words, &scale, zero.t, bias.t, res.t});
   const Where w(x, a[11]);
   at::Tensor x2 = dims == 2 ? x : x.reshape({-1, K}), r2;
-  if (x2.stride(1) != 1 || x2.stride(0) % 8 != 0 || ((uintptr_t)x2.data_ptr() & 15))
-    x2 = x2.clone(at::MemoryFormat::Contiguous);             // rows the kernel cannot load 16 bytes at a time
+  if (x2.stride(1) != 1 || x2.stride(0) % 8 != 0 || x2.stride(0) >= 1 << 24 || ((uintptr_t)x2.data_ptr() & 15))
+    x2 = x2.clone(at::MemoryFormat::Contiguous);             // rows the kernel cannot load 16 bytes at a time or address
   if (res) {
     r2 = dims == 2 ? *res.t : res->reshape({-1, N});
     if (r2.stride(1) != 1) r2 = r2.contiguous();

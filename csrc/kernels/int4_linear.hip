@@ -238,7 +238,7 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(const Int4Args a) {
         use_step<T, S>(y, w1, t1);
       }
     }
-    const bool tail = full < s1 && kw == (full - s0) % a.kw;
+    const bool tail = full >= s0 && full < s1 && kw == (full - s0) % a.kw;
     if (tail) {
       load_words<R>(w0, a, full, tile0, tiles, Ks, lane);
       load_rest_tail<R, CT, G>(t0, a, zero, x, xo, full, tile0, tiles, g);
@@ -305,18 +305,16 @@ template <typename T, typename S>
 static void launch4_r(const Int4Args& a, int R, int CT, int G, int nw, hipStream_t stream) {
   if (CT == 1) {
     if (R == 1) launch4_g<T, S, 1, 1>(a, G, nw, stream);
-    else if (R == 2) launch4_g<T, S, 2, 1>(a, G, nw, stream);
-    else launch4_g<T, S, 4, 1>(a, G, nw, stream);
+    else launch4_g<T, S, 2, 1>(a, G, nw, stream);
   } else {
     if (R == 1) launch4_g<T, S, 1, 2>(a, G, nw, stream);
-    else if (R == 2) launch4_g<T, S, 2, 2>(a, G, nw, stream);
     else launch4_g<T, S, 4, 2>(a, G, nw, stream);
   }
 }
 
 // x: [M, K] (row stride given), y: [M, N] contiguous.  dtype, sdtype: 0 bf16, 1 fp16.  K % G == 0, G 32, 64 or 128.
-// A wave holds `tiles` (1, 2, 4) tiles of 16 outputs, a workgroup nw x kw <= 8 waves, K is split into kz parts over workgroups
-// (part: [kz][M][N rounded up to 16] floats where kz > 1).
+// A wave holds `tiles` tiles of 16 outputs (1, or 2 up to 16 rows and 4 from there), a workgroup nw x kw <= 8 waves, K is split
+// into kz parts over workgroups (part: [kz][M][N rounded up to 16] floats where kz > 1).
 extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, const void* scale, const void* zero,
                                  const void* bias, const void* res, long long res_rs, void* y, int M, int N, int K, int G,
                                  int act, int dtype, int sdtype, int tiles, int nw, int kw, int kz, void* part,
@@ -329,7 +327,7 @@ extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, c
   if (act != ACT_NONE && act != ACT_RELU && act != ACT_GELU) return -4;
   const int CT = M <= 16 ? 1 : 2;
   if ((M + 16 * CT - 1) / (16 * CT) > 65535) return -5;
-  if ((tiles != 1 && tiles != 2 && tiles != 4) || nw < 1 || kw < 1 || nw * kw > 8 || nw * kw * tiles * CT > 64) return -6;
+  if ((tiles != 1 && tiles != 2 * CT) || nw < 1 || kw < 1 || nw * kw > 8 || nw * kw * tiles * CT > 64) return -6;
   if (kz < 1 || kz > 64 || (kz > 1 && (!part || ((uintptr_t)part & 15) || part_floats < (long long)kz * M * ((N + 15) / 16 * 16)))) return -7;
   if ((long long)M * ((N + 15) / 16 * 4) > 0x7fffffffLL * 256) return -8;
   Int4Args a{x, (const uint32_t*)w, scale, (const uint8_t*)zero, (const float*)bias, res, y, x_rs, res_rs, (float*)part,
