@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../kernels/decode_abi.h"
@@ -79,6 +80,12 @@ void same_device(const c10::Device& d, std::initializer_list<const at::Tensor*> 
   for (const at::Tensor* t : ts) need(!t || t->device() == d, "all tensors live on one device");
 }
 
+// The operators have no backward: a result that silently carried no gradient would train nothing.
+void no_gradient(std::initializer_list<const at::Tensor*> ts) {
+  if (c10::GradMode::is_enabled())
+    for (const at::Tensor* t : ts) need(!t || !t->requires_grad(), "the operator has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+
 int half_type(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : -1; }
 
 void check_cache(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& table, const at::Tensor& lens) {
@@ -106,10 +113,11 @@ PyObject* append(PyObject* const* a) {
   const at::ScalarType dt = kp.scalar_type();
   need(k.scalar_type() == dt && v.scalar_type() == dt && k.stride(2) == 1 && v.stride(2) == 1,
        "k and v have the cache's type and a contiguous last dimension");
-  need(D % 8 == 0, "D is a multiple of 8");
+  need(D % 8 == 0 && hkv > 0, "D is a multiple of 8, the cache has heads");
+  no_gradient({&k, &v, &kp, &vp, q.t});
   same_device(k.device(), {&v, &kp, &vp, &table, &lens, q.t, cos.t, sin.t, starts.t});
   if (q)
-    need(q->dim() == 3 && q->size(0) == T && q->size(2) == D && q->scalar_type() == dt && q->stride(2) == 1,
+    need(q->dim() == 3 && q->size(0) == T && q->size(1) > 0 && q->size(2) == D && q->scalar_type() == dt && q->stride(2) == 1,
          "q is [T, heads, D] of the cache's type and device with a contiguous last dimension");
   need((bool)cos == (bool)sin, "cos and sin come together");
   int64_t rot = 0;
@@ -165,6 +173,7 @@ PyObject* attention(PyObject* const* a) {
   need(table.size(0) == B && kp.size(3) == D && hkv > 0 && hq % hkv == 0,
        "q, table and cache disagree: one table row per sequence, D alike, heads a multiple of kv_heads");
   need(page > 0 && page % 16 == 0 && (D == 64 || D == 128), "page is a multiple of 16, D is 64 or 128");
+  no_gradient({&q, &kp, &vp});
   same_device(q.device(), {&kp, &vp, &table, &lens});
   double scale = 1.0 / std::sqrt((double)D);
   if (a[5] != Py_None) {

@@ -84,6 +84,12 @@ def bind():
     return _BIND
 
 
+def no_gradient(*ts: Optional[torch.Tensor]) -> None:
+    """For operators without a backward: a result that silently carried no gradient would train nothing."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise ValueError("the operator has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
 def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
     if t is None:
         return ctypes.c_void_p(0)

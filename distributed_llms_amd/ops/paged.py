@@ -17,7 +17,8 @@ accepted plus one - the rejected tokens' slots are simply written again).
 * What lies in slots nobody has written (NaN included) does not reach any result.
 
 Everything runs on the current stream of the tensors' device, allocates only through PyTorch and reads no device value on
-the host, so a decode step can be captured in a hipGraph and replayed while ``lens`` advances.
+the host, so a decode step can be captured in a hipGraph and replayed while ``lens`` advances.  Neither operator has a
+gradient; tensors that require one are refused outside torch.no_grad().
 """
 from __future__ import annotations
 
@@ -122,11 +123,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     T = k.shape[0]
     if k.dtype != dt or v.dtype != dt or k.stride(2) != 1 or v.stride(2) != 1:
         raise ValueError("k and v have the cache's type and a contiguous last dimension")
-    if D % 8 != 0:
-        raise ValueError("D is a multiple of 8")
+    if D % 8 != 0 or hkv == 0:
+        raise ValueError("D is a multiple of 8, the cache has heads")
+    _loader.no_gradient(k, v, k_pages, v_pages, q)
     if any(x is not None and x.device != k.device for x in (v, k_pages, v_pages, table, lens, q, cos, sin, starts)):
         raise ValueError("all tensors live on one device")
-    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != dt or q.stride(2) != 1):
+    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[1] == 0 or q.shape[2] != D or q.dtype != dt or q.stride(2) != 1):
         raise ValueError("q is [T, heads, D] of the cache's type and device with a contiguous last dimension")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
@@ -198,6 +200,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("q, table and cache disagree: one table row per sequence, D alike, heads a multiple of kv_heads")
     if page % 16 != 0 or page == 0 or D not in (64, 128):
         raise ValueError("page is a multiple of 16, D is 64 or 128")
+    _loader.no_gradient(q, k_pages, v_pages)
     if any(x.device != q.device for x in (k_pages, v_pages, table, lens)):
         raise ValueError("all tensors live on one device")
     o, lse = paged_attention_reference(q, k_pages, v_pages, table, lens, scale, causal)

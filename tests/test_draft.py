@@ -168,3 +168,51 @@ def test_refuses(why):
     REFUSED[why](c)
     with pytest.raises(ValueError):
         verify_draft(**c)
+
+
+@pytest.mark.parametrize("dev", ["checks", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("why", sorted(REFUSED))
+def test_refuses_on_the_device_path(why, dev):
+    """The host side for device tensors refuses before it launches, so its checks can be seen without a GPU too."""
+    from distributed_llms_amd.ops import _loader
+
+    if dev == "checks" and not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    c = case(1, 2, 3, 10, torch.float32)
+    REFUSED[why](c)
+    d = on(c, "cuda" if dev == "cuda" else "cpu")
+    args = [d[x] for x in ("draft", "target", "u", "proposal", "counts")]
+    with pytest.raises(ValueError):
+        _loader.bind().verify_draft(*args, -1, None, 0)
+    with pytest.raises(ValueError):
+        _loader.bind().verify_draft(*args, 1 << 40, None, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pieces", [1, 2, 7, 48, 64])
+@pytest.mark.parametrize("k", [2, 4, 5, 6, 9, 11, 13, 16])
+def test_rows_in_pieces(k, pieces, monkeypatch):
+    """Any number of pieces, also more than there are tokens."""
+    from distributed_llms_amd.ops import draft as D
+
+    monkeypatch.setattr(D, "_PIECES", pieces)
+    B, n, V, dt, proposal, ragged = CASES[k]
+    c = case(100 * k, min(B, 40), n, V, DTYPES[dt], proposal, ragged)
+    same(verify_draft(**on(c, "cuda")), plain(**c))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pieces", [1, 2, 7, 48, 64])
+@pytest.mark.parametrize("V", [64, 700, 5000, 12000])
+def test_the_last_token_stands_for_the_end_of_the_row(V, pieces, monkeypatch):
+    """u = 1: no cumulative weight lies beyond it, so the last token with weight is the answer whatever the sums' rounding;
+    weights end at another token in every sequence."""
+    from distributed_llms_amd.ops import draft as D
+
+    monkeypatch.setattr(D, "_PIECES", pieces)
+    g = torch.Generator().manual_seed(V)
+    p = torch.rand(60, 1, V, generator=g) + 1e-3
+    last = torch.randint(0, V, (60,), generator=g)
+    p[torch.arange(V)[None, None] > last[:, None, None]] = 0.0
+    tokens, accepted = verify_draft(torch.zeros(60, 0, dtype=torch.int32, device="cuda"), p.cuda(), torch.ones(60, 1, device="cuda"))
+    assert torch.equal(tokens.cpu()[:, 0].long(), last) and not bool(accepted.any())

@@ -177,3 +177,60 @@ def test_refuses_to_pack():
     for bad in (dict(group=48), dict(weight=torch.zeros(4, 100)), dict(weight=torch.zeros(4))):
         with pytest.raises(ValueError):
             Q.quantize_int4(**{"weight": torch.zeros(4, 128), "group": 64, **bad})
+
+
+MORE_REFUSED = {
+    **REFUSED,
+    "rows that require a gradient": lambda c: c.update(x=c["x"].clone().requires_grad_()),
+    "a bias that requires a gradient": lambda c: c.update(bias=torch.zeros(40, requires_grad=True)),
+}
+
+
+@pytest.mark.parametrize("dev", ["checks", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("why", sorted(set(MORE_REFUSED) - {"an unknown activation"}))
+def test_refuses_on_the_device_path(why, dev):
+    """The host side for device tensors refuses before it launches, so its checks can be seen without a GPU too."""
+    from distributed_llms_amd.ops import _loader
+
+    if dev == "checks" and not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    c = dict(x=torch.zeros(2, 64, dtype=torch.bfloat16), w=layer(0, 40, 64, 32, False, torch.bfloat16)[3], bias=None, res=None)
+    MORE_REFUSED[why](c)
+    with pytest.raises(ValueError):
+        Q.linear_int4(**c)
+    to_dev = "cuda" if dev == "cuda" else "cpu"
+    (x, bias, res), w = to(to_dev, c["x"], c["bias"], c["res"]), c["w"].to(to_dev)
+    with pytest.raises(ValueError):
+        _loader.bind().linear_int4(x, w.words, w.scale, w.zero, w.n, w.k, w.group, bias, 0, res, None, 0)
+
+
+SHAPES = [  # tiles of a wave (None: the wide one of the row count), waves over outputs, waves over K, parts of K
+    (1, 1, 8, 1), (1, 2, 4, 3), (1, 4, 2, 64), (None, 1, 4, 1), (None, 2, 2, 2), (None, 1, 4, 5), (None, 1, 1, 4),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("i", [2, 3, 4, 5, 7, 8, 10])
+def test_every_launch_shape_is_right(i, shape, monkeypatch):
+    """Waves and parts of K that get no features at all included."""
+    rows, n, k, group, zero, act, has_bias, has_res, dt, sdt = CASES[i]
+    monkeypatch.setattr(Q, "_SHAPE", (shape[0] or (2 if rows <= 16 else 4), *shape[1:]))
+    codes, scale, z, w = layer(i, n, k, group, zero, DTYPES[sdt])
+    g = torch.Generator().manual_seed(50 + i)
+    x = torch.randn(rows, k, generator=g).to(DTYPES[dt])
+    bias = torch.randn(n, generator=g) if has_bias else None
+    res = torch.randn(rows, n, generator=g).to(DTYPES[dt]) if has_res else None
+    xd, bd, rd = to("cuda", x, bias, res)
+    check(Q.linear_int4(xd, w.to("cuda"), bd, act=act, res=rd).cpu(), x, codes, scale, z, group, bias, act, res)
+
+
+@pytest.mark.gpu
+def test_rows_too_far_apart_are_gathered():
+    """x as every 2^24-th element row of a long buffer."""
+    codes, scale, z, w = layer(1, 70, 128, 64, False, torch.bfloat16)
+    big = torch.zeros((1 << 24) + 128, dtype=torch.bfloat16, device="cuda")
+    x = torch.randn(2, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    rows = big.as_strided((2, 128), (1 << 24, 1))
+    rows.copy_(x)
+    check(Q.linear_int4(rows, w.to("cuda")).cpu(), x, codes, scale, z, 64, None, "none", None)

@@ -491,3 +491,67 @@ def test_kernels_refuse_what_they_cannot_load():
         P.paged_append(odd, odd, d["k_pages"], d["v_pages"], d["table"], d["lens"])
     with pytest.raises(ValueError):
         P.paged_append(odd.cpu(), odd.cpu(), d["k_pages"], d["v_pages"], d["table"], d["lens"])
+
+
+BINDING = ["checks", pytest.param("cuda", marks=pytest.mark.gpu)]     # "checks": the device path's host checks, on CPU tensors
+
+
+def refused_by_the_binding(dev, c, call):
+    """The host side for device tensors refuses before it launches, so its checks can be seen without a GPU too."""
+    from distributed_llms_amd.ops import _loader
+
+    if dev == "checks" and not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    with pytest.raises(ValueError):
+        call(_loader.bind(), {n: x.cuda() if dev == "cuda" and torch.is_tensor(x) else x for n, x in c.items()})
+
+
+MORE_APPEND_REFUSED = {
+    **APPEND_REFUSED,
+    "keys that require a gradient": lambda c: c.update(k=c["k"].clone().requires_grad_()),
+    "queries that require a gradient": lambda c: c.update(q=c["q"].clone().requires_grad_()),
+    "a cache without heads": lambda c: c.update(k=c["k"][:, :0], v=c["v"][:, :0], k_pages=c["k_pages"][:, :, :0], v_pages=c["v_pages"][:, :, :0]),
+    "queries without heads": lambda c: c.update(q=c["q"][:, :0]),
+}
+MORE_ATT_REFUSED = {
+    **ATT_REFUSED,
+    "queries that require a gradient": lambda c: c.update(q=c["q"].clone().requires_grad_()),
+    "a cache that requires a gradient": lambda c: c.update(v_pages=c["v_pages"].clone().requires_grad_()),
+}
+
+
+@pytest.mark.parametrize("dev", BINDING)
+@pytest.mark.parametrize("why", sorted(MORE_APPEND_REFUSED))
+def test_append_refuses_on_the_device_path(why, dev):
+    c = {"q": None, "cos": None, "sin": None, "starts": None, "interleaved": False, **_append_args()}
+    MORE_APPEND_REFUSED[why](c)
+    with pytest.raises(ValueError):
+        P.paged_append(**c)
+    refused_by_the_binding(dev, c, lambda bind, d: bind.paged_append(
+        *(d[x] for x in ("k", "v", "k_pages", "v_pages", "table", "lens", "q", "cos", "sin", "starts", "interleaved")), 0))
+
+
+@pytest.mark.parametrize("dev", BINDING)
+@pytest.mark.parametrize("why", sorted(MORE_ATT_REFUSED))
+def test_attention_refuses_on_the_device_path(why, dev):
+    c = {"scale": None, "causal": True, **att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True)}
+    MORE_ATT_REFUSED[why](c)
+    with pytest.raises(ValueError):
+        P.paged_attention(**c)
+    refused_by_the_binding(dev, c, lambda bind, d: bind.paged_attention(
+        *(d[x] for x in ("q", "k_pages", "v_pages", "table", "lens", "scale", "causal")), None, False, None, 0, 0))
+
+
+@pytest.mark.parametrize("dev", BINDING)
+def test_the_device_path_wants_tensors_and_numbers(dev):
+    c = {"scale": None, "causal": True, **att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True)}
+    for bad in (dict(scale="large"), dict(q=3), dict(lens=None)):
+        refused_by_the_binding(dev, {**c, **bad}, lambda bind, d: bind.paged_attention(
+            *(d[x] for x in ("q", "k_pages", "v_pages", "table", "lens", "scale", "causal")), None, False, None, 0, 0))
+
+
+def test_no_gradient_is_asked_for_under_no_grad():
+    c = att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True)
+    want = P.paged_attention(**c)
+    with torch.no_grad():
+        assert torch.equal(P.paged_attention(**{**c, "q": c["q"].clone().requires_grad_()}), want)
