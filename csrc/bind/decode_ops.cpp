@@ -207,9 +207,9 @@ PyObject* attention(PyObject* const* a) {
 
 // ------------------------------------------------------------------------------------------ verification
 // Workgroups that share a sequence's row of `bytes` (target's and proposal's).  Up to 8192 tokens one holds it in registers
-// (8 x 4000: 5.7 us, 8.7 in pieces).  128 short rows keep the card busy by themselves (256 x 32000 bf16: 15.3 us, in pieces
-// 16.7), long ones are dealt out more evenly in pieces (192 x 50265 fp32: 21.6 us in 32, 23.3 in one; 512 x 50265: 38.8 and
-// 45.9).  Fewer rows than compute units want more pieces (1 x 50265: 8.3 us in 48, 17.6 in one).
+// (8 x 4000: 5.8 us, 8.0 in pieces).  128 short rows keep the card busy by themselves (256 x 32000 bf16: 14.5 us, in pieces
+// 15.7), long ones are dealt out more evenly in pieces (192 x 50265 fp32: 21.0 us in 32, 21.6 in one; 512 x 50265: 38.4 and
+// 42.9).  Fewer rows than compute units want more pieces (1 x 50265: 8.0 us in 48, 17 in one).
 int64_t pieces_of(int64_t B, int64_t V, int64_t bytes) {
   if (V <= 8192 || (B >= 128 && bytes < 256 << 10) || B > 65535) return 1;
   return B < 32 ? std::min<int64_t>(48, (V + 511) / 512) : std::min<int64_t>(32, (V + 1535) / 1536);

@@ -161,6 +161,20 @@ __device__ __forceinline__ void find_border(const Rest<T>& r, int lo, int hi, bo
   if (found >= 0) atomicMin(&hit[0], found);
   else if (last >= 0) atomicMax(&hit[1], last);
 }
+__device__ __forceinline__ void find_border(const double (&w)[8], int lo, double before, double mine, double x, int* hit) {
+  if (!(mine > 0.0) || before > x) return;
+  int found = -1, last = -1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    before += w[i];
+    if (w[i] > 0.0) {
+      last = lo + i;
+      if (before > x && found < 0) found = lo + i;
+    }
+  }
+  if (found >= 0) atomicMin(&hit[0], found);
+  else atomicMax(&hit[1], last);
+}
 __device__ __forceinline__ int hit_of(const int* hit) { return hit[0] < 0x7fffffff ? hit[0] : max(hit[1], 0); }
 
 // One workgroup per sequence, the whole row in registers: wave w holds U x 64 consecutive weights, U of them a lane.
@@ -228,10 +242,24 @@ template <typename T, int WAVES>
 __device__ __forceinline__ void find_in_piece(const Rest<T>& r, int p0, int p1, bool all, double before, double x, int lane,
                                               int wave, double* s_w, int* s_hit) {
   const int per = (p1 - p0 + 64 * WAVES - 1) / (64 * WAVES), lo = min(p0 + (int)threadIdx.x * per, p1), hi = min(lo + per, p1);
-  double rest, whole, sum;
-  sum_weights(r, lo, hi, 1, rest, whole);
-  const double mine = all ? whole : rest, prior = sum_before<WAVES>(mine, lane, wave, s_w, sum);
-  find_border(r, lo, hi, all, before + prior, mine, x, s_hit);
+  double sum;
+  if (per <= 8) {                                            // read once: 1 x 50265 8.0 us, read twice 8.5
+    double w[8], full[8], mine = 0.0;
+    if (r.q) weights_of<T, true, 8>(r, lo, hi, 1, w, full);
+    else weights_of<T, false, 8>(r, lo, hi, 1, w, full);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = all ? full[i] : w[i];
+      mine += w[i];
+    }
+    const double prior = sum_before<WAVES>(mine, lane, wave, s_w, sum);
+    find_border(w, lo, before + prior, mine, x, s_hit);
+  } else {
+    double rest, whole;
+    sum_weights(r, lo, hi, 1, rest, whole);
+    const double mine = all ? whole : rest, prior = sum_before<WAVES>(mine, lane, wave, s_w, sum);
+    find_border(r, lo, hi, all, before + prior, mine, x, s_hit);
+  }
 }
 
 // One workgroup per sequence: a wave sums a contiguous piece of the row, then all of them look for the border in the piece
