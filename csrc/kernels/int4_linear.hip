@@ -15,6 +15,10 @@
 //
 // The waves of a workgroup share R tiles of 16 outputs and split K between them, 128 features at a time; their sums meet in
 // LDS.  The next step's loads are in flight while a step is computed.
+//
+// 5 x 50265 x 1024: 9.5 us, 2.9 TB/s; 1 x 16384 x 4096: 10.2 us; 24 x 8192 x 28672: 39 us, 3.2 TB/s.  There a stream of the
+// words alone takes 26 us; fetching x (from L2), the scales and the unpacking, scaling and products cost 4 to 8 us each on top,
+// which neither x through LDS for eight waves (40 - 46 us), nor more waves over K (44) or over outputs (41 - 42) hid.
 #include "common.h"
 #include "decode_abi.h"
 
