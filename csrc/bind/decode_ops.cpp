@@ -182,12 +182,14 @@ PyObject* attention(PyObject* const* a) {
       PyErr_Clear();
       throw Refused("scale is a number");
     }
+    need(std::isfinite((float)scale), "scale is a finite number");
   }
   int64_t bound = width * page;
   if (a[7] != Py_None) bound = std::min<int64_t>(bound, number(a[7]));
   const int64_t all = n * (hq / hkv), groups = all <= 48 ? 1 : (all + 31) / 32, rows = (all + groups - 1) / groups;
   const int64_t problems = B * hkv * groups;
-  const Deal d = a[9] == Py_None ? deal_out(problems, rows, bound, D) : Deal{number(a[9]), number(a[10])};
+  Deal d = a[9] == Py_None ? deal_out(problems, rows, bound, D) : Deal{number(a[9]), number(a[10])};
+  if (n * hq >= (int64_t)(1 << 24) / std::max<int64_t>(B, 1)) d = {0, 0};     // the join's launch ends there, and the card is full
   const Where w(q, a[11]);
   at::Tensor o = at::empty({B, n, hq, D}, q.options()), lse, part;
   const bool want = truth(a[8]);
@@ -293,6 +295,10 @@ PyObject* int4(PyObject* const* a) {
     need(res->dim() == dims && res->size(dims - 1) == N && res->sizes().slice(0, dims - 1) == x.sizes().slice(0, dims - 1) &&
              res->scalar_type() == x.scalar_type(),
          "res is [..., N] of x's type");
+  need(G > 0 && K % G == 0 && words.scalar_type() == at::kInt && words.is_contiguous() && words.numel() == (N + 15) / 16 * ((K + 127) / 128) * 256 &&
+           half_type(scale.scalar_type()) >= 0 && scale.is_contiguous() && scale.numel() == K / G * ((N + 15) / 16 * 16) &&
+           (!zero || (zero->scalar_type() == at::kByte && zero->is_contiguous() && zero->numel() == scale.numel())),
+       "words, scale and zero are not those of an [N, K] layer as pack_int4 lays it out");
   no_gradient({&x, bias.t, res.t});
   same_device(x.device(), {&words, &scale, zero.t, bias.t, res.t});
   const Where w(x, a[11]);

@@ -403,7 +403,7 @@ extern "C" int dlamd_verify_draft(const void* draft, long long d_bs, const void*
                                   const void* counts, void* tokens, void* accepted, void* sums, long long sums_doubles, int pieces, int B, int n,
                                   int V, int pad, int dtype, hipStream_t stream) {
   if (B <= 0) return 0;
-  if (n < 0 || n > 63 || V <= 0 || V >= 0x40000000) return -1;
+  if (n < 0 || n > 63 || V <= 0 || V >= 0x40000000 || B >= 1 << 22) return -1;      // a launch has fewer than 2^32 threads
   if (pieces < 1 || pieces > 64 || (pieces > 1 && (B > 65535 || !sums || ((uintptr_t)sums & 7) || sums_doubles < 2LL * B * pieces))) return -3;
   VerifyArgs a{(const int*)draft, p, q, (const float*)u, (const int*)counts, (int*)tokens, (int*)accepted, d_bs, p_bs, p_ns,
                q_bs, q_ns, u_bs, (double*)sums, B, n, V, pad, pieces};

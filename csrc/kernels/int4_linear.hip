@@ -324,7 +324,7 @@ extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, c
                                  int act, int dtype, int sdtype, int tiles, int nw, int kw, int kz, void* part,
                                  long long part_floats, hipStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || (G != 32 && G != 64 && G != 128) || K % G != 0 || N > 0x7ffffff0) return -1;
+  if (K <= 0 || (G != 32 && G != 64 && G != 128) || K % G != 0 || N > 1 << 26) return -1;
   if (x_rs < 0 || x_rs >= (1 << 24) || K >= (1 << 24)) return -9;   // a workgroup's 32 rows of x: 31-bit offsets
   if (x_rs % 8 != 0 || (((uintptr_t)x | (uintptr_t)w) & 15) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3) || ((uintptr_t)y & 7)) return -2;
   if ((dtype != 0 && dtype != 1) || (sdtype != 0 && sdtype != 1)) return -3;
@@ -333,7 +333,7 @@ extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, c
   if ((M + 16 * CT - 1) / (16 * CT) > 65535) return -5;
   if ((tiles != 1 && tiles != 2 * CT) || nw < 1 || kw < 1 || nw * kw > 8 || nw * kw * tiles * CT > 64) return -6;
   if (kz < 1 || kz > 64 || (kz > 1 && (!part || ((uintptr_t)part & 15) || part_floats < (long long)kz * M * ((N + 15) / 16 * 16)))) return -7;
-  if ((long long)M * ((N + 15) / 16 * 4) > 0x7fffffffLL * 256) return -8;
+  if (kz > 1 && (long long)M * ((N + 15) / 16 * 4) > 0xffffff00LL) return -8;      // a launch has fewer than 2^32 threads
   Int4Args a{x, (const uint32_t*)w, scale, (const uint8_t*)zero, (const float*)bias, res, y, x_rs, res_rs, (float*)part,
              M, N, K, act, kw, kz, zero ? 1 : 0};
   if (dtype == 0 && sdtype == 0) launch4_r<bf16_t, bf16_t>(a, tiles, CT, G, nw, stream);

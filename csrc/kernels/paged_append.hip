@@ -140,6 +140,7 @@ extern "C" int dlamd_paged_append(const void* k, long long k_ts, long long k_hs,
   if ((k_ts | k_hs | v_ts | v_hs | kp_ps | kp_ss | kp_hs | vp_ps | vp_ss | vp_hs) % 8 != 0 || (q && (q_ts | q_hs) % 8 != 0)) return -5;
   if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)qo | (uintptr_t)kp | (uintptr_t)vp) & 15) return -6;
   if (dtype != 0 && dtype != 1) return -7;
+  if (T >= 1 << 24) return -8;                               // a launch has fewer than 2^32 threads
   AppendArgs a{k, v, q, kp, vp, qo, (const int*)table, (const int*)lens, (const int*)starts, (const float*)cs, (const float*)sn,
                k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, kp_ps, kp_ss, kp_hs, vp_ps, vp_ss, vp_hs, t_bs,
                B, T, starts ? 0 : T / B, Hq, Hkv, D, rot, page, width, pages, interleaved};

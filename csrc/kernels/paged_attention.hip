@@ -606,13 +606,14 @@ extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_
   if ((long long)width * page > 0x7ff00000LL || (long long)width * (page / 16) * (page / 16) >= (1LL << 32)) return -5;
   if (dtype != 0 && dtype != 1) return -6;
   if (share < 0 || share > (1 << 20) || (share > 0 && (least < 1 || !part || ((uintptr_t)part & 15)))) return -7;
-  if ((long long)n * Hq > 0x7fffffffLL || (long long)B * n * Hq > 0x7fffffffLL) return -9;
+  if ((long long)n * Hq > 0x7fffffffLL || (share > 0 && (long long)n * Hq >= (1LL << 24) / B)) return -9;   // the join: a workgroup per row
   // Rows of one problem, in tiles of 16.  Up to 48 share a key's fetch (12 ragged caches, 40 rows: 26 us; as two groups that
   // fetch it twice 31); beyond, groups of up to 32 (64 rows in one wave: 30 us for 2 x 16384 keys, in two groups 26.5: the
   // registers of more rows leave one workgroup per compute unit).
   const int R = n * (Hq / Hkv), groups = R <= 48 ? 1 : (R + 31) / 32, rows = (R + groups - 1) / groups;
   if (share > 0 && part_floats < ((long long)share + (long long)B * Hkv * groups) * rows * (D + 4)) return -12;
-  // problems, parts and tiles are counted in 32 bits
+  // problems, parts and tiles are counted in 32 bits, the launch in 2^24 workgroups
+  if ((long long)B * Hkv * groups + share >= (1LL << 24)) return -10;
   if (((long long)B * Hkv * groups + share) * ((long long)width * page / 64 + 2) > 0x7fffffffLL) return -10;
   if (width == 0) {                                          // no table to read: one entry of anything, and no pages
     table = lens;

@@ -87,7 +87,10 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, symmetric: bool = True
     w = weight.detach().float().view(N, K // group, group)
     hi, lo = w.amax(-1).clamp(min=0.0), w.amin(-1).clamp(max=0.0)
     s = torch.maximum(hi / 7.0, -lo / 8.0) if symmetric else (hi - lo) / 15.0
-    s = torch.where(s > 0, s, torch.ones_like(s)).to(scale_dtype)
+    s = s.to(scale_dtype)
+    if not bool(torch.isfinite(s).all()):
+        raise ValueError("weights are finite and their scales fit scale_dtype")
+    s = torch.where(s > 0, s, torch.ones_like(s))                                  # groups of zeros, or of less than a scale can say
     sf = s.float()
     z = torch.full_like(sf, 8.0) if symmetric else (-lo / sf).round().clamp(0, 15)
     c = ((w / sf[..., None]).round() + z[..., None]).clamp(0, 15).to(torch.uint8).view(N, K)

@@ -168,6 +168,7 @@ def paged_attention_reference(q, k_pages, v_pages, table, lens, scale: Optional[
             x = torch.matmul(q[b, i].to(dtype).reshape(hkv, hq // hkv, D), k) * scale
             lse[b, i] = torch.logsumexp(x, -1).reshape(hq)
             o[b, i] = torch.matmul(torch.softmax(x, -1), v).reshape(hq, D)
+            o[b, i, torch.isneginf(lse[b, i])] = 0.0                              # no score above -inf: nothing seen
     return o, lse
 
 
@@ -185,7 +186,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     ``causal``: token i of a sequence sees the positions up to its own, lens[b] + i (its key is in the cache already:
     ``paged_append`` ran with the same ``lens``).  Not causal: every query sees exactly the lens[b] kept positions
-    (cross-attention over encoder tokens held in pages).  A query that sees nothing gives 0 and a log-sum-exp of -inf.
+    (cross-attention over encoder tokens held in pages).  A query that sees nothing, or only scores of -inf, gives 0 and a
+    log-sum-exp of -inf.
     ``max_len``: an upper bound of the positions any query sees, when the caller knows a tighter one than ``width * page``
     (only used to choose how the work is split; lengths are read on the device).  D is 64 or 128, page % 16 == 0."""
     if q.is_cuda:
@@ -200,6 +202,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("q, table and cache disagree: one table row per sequence, D alike, heads a multiple of kv_heads")
     if page % 16 != 0 or page == 0 or D not in (64, 128):
         raise ValueError("page is a multiple of 16, D is 64 or 128")
+    if scale is not None and not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError("scale is a finite number")
     _loader.no_gradient(q, k_pages, v_pages)
     if any(x.device != q.device for x in (k_pages, v_pages, table, lens)):
         raise ValueError("all tensors live on one device")

@@ -234,3 +234,31 @@ def test_rows_too_far_apart_are_gathered():
     rows = big.as_strided((2, 128), (1 << 24, 1))
     rows.copy_(x)
     check(Q.linear_int4(rows, w.to("cuda")).cpu(), x, codes, scale, z, 64, None, "none", None)
+
+
+def test_quantize_keeps_to_what_scales_can_say():
+    w = torch.zeros(3, 64)
+    w[0, 5], w[1, 40] = 1e-9, 3.0
+    q = Q.quantize_int4(w, 32, scale_dtype=torch.float16)            # 1e-9 / 7 is no fp16 number
+    d = q.dequantize()
+    assert bool((d[0] == 0).all()) and bool((d[2] == 0).all()) and abs(float(d[1, 40]) - 3.0) <= 3.0 * 2.0 ** -11
+    for bad, dt in ((1e7, torch.float16), (math.inf, torch.bfloat16), (math.nan, torch.bfloat16)):
+        w[1, 40] = bad
+        with pytest.raises(ValueError):
+            Q.quantize_int4(w, 32, scale_dtype=dt)
+
+
+@pytest.mark.parametrize("dev", ["checks", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("change", [dict(n=41 + 16), dict(k=256), dict(group=64), dict(group=0), dict(n=1)], ids=str)
+def test_refuses_weights_of_another_layout(change, dev):
+    """A layer whose sizes do not fit its words, scales and zeros is refused before it launches."""
+    import dataclasses
+
+    from distributed_llms_amd.ops import _loader
+
+    if dev == "checks" and not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    w = dataclasses.replace(layer(0, 40, 128, 32, True, torch.bfloat16)[3].to("cuda" if dev == "cuda" else "cpu"), **change)
+    x = torch.zeros(2, w.k, dtype=torch.bfloat16, device=w.words.device)
+    with pytest.raises(ValueError):
+        _loader.bind().linear_int4(x, w.words, w.scale, w.zero, w.n, w.k, w.group, None, 0, None, None, 0)

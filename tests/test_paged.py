@@ -517,6 +517,9 @@ MORE_ATT_REFUSED = {
     **ATT_REFUSED,
     "queries that require a gradient": lambda c: c.update(q=c["q"].clone().requires_grad_()),
     "a cache that requires a gradient": lambda c: c.update(v_pages=c["v_pages"].clone().requires_grad_()),
+    "an infinite scale": lambda c: c.update(scale=math.inf),
+    "no scale at all": lambda c: c.update(scale=math.nan),
+    "a scale beyond fp32": lambda c: c.update(scale=1e39),
 }
 
 
@@ -555,3 +558,53 @@ def test_no_gradient_is_asked_for_under_no_grad():
     want = P.paged_attention(**c)
     with torch.no_grad():
         assert torch.equal(P.paged_attention(**{**c, "q": c["q"].clone().requires_grad_()}), want)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_row_with_nothing_but_scores_of_minus_infinity(dev):
+    """As if it saw nothing; the row of the next token sees one key more, and only that."""
+    c = att_case(6, [1, 40], 2, 16, 2, 2, 64, torch.bfloat16, True)
+    c["q"] = (c["q"].abs() + 0.1).to(torch.bfloat16)
+    for pos in (0, 1):
+        c["k_pages"][int(c["table"][0, 0]), pos] = float("-inf")
+    first = c["lens"].clone()
+    first[0] = 0
+    for lens in (c["lens"], first):
+        c["lens"] = lens
+        d = {x: y.to(dev) if torch.is_tensor(y) else y for x, y in c.items()}
+        o, lse = P.paged_attention(**d, return_lse=True)
+        ref, ref_lse = P.paged_attention_reference(**c, dtype=torch.float64)
+        rows = 2 - int(lens[0])                                      # those that see positions 0 and 1 at most
+        assert bool((o[0, :rows].cpu() == 0).all()) and bool(torch.isneginf(lse[0, :rows].cpu()).all())
+        assert bool(((o.cpu().double() - ref).abs() <= att_tolerance(c, ref)).all())
+    c["k_pages"][int(c["table"][0, 0]), 1] = 0.5
+    d = {x: y.to(dev) if torch.is_tensor(y) else y for x, y in c.items()}
+    o = P.paged_attention(**d).cpu()
+    assert bool((o[0, 0] == 0).all()) and torch.equal(o[0, 1], c["v_pages"][int(c["table"][0, 0]), 1])
+
+
+def test_c_entries_refuse_more_than_a_launch_holds():
+    """Sizes whose grids would have 2^32 threads, and workspaces that are too small; refused before anything is read."""
+    import ctypes
+
+    from distributed_llms_amd.ops import _loader
+
+    if not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    lib = _loader.lib()
+    i, ll, p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
+    z, at = p(0), p(1 << 20)
+
+    def append(T):
+        return lib.dlamd_paged_append(at, ll(64), ll(64), at, ll(64), ll(64), z, ll(0), ll(0), z, at, ll(1024), ll(64), ll(64), at, ll(1024),
+                                      ll(64), ll(64), at, ll(1), at, z, z, z, i(1), i(T), i(0), i(1), i(64), i(0), i(16), i(1), i(0), i(0),
+                                      i(0), z)
+
+    def attention(B, n, share, floats):
+        return lib.dlamd_paged_attention(at, ll(64), ll(64), ll(64), at, ll(1024), ll(64), ll(64), at, ll(1024), ll(64), ll(64), at, ll(1),
+                                         at, at, z, at, ll(floats), i(share), i(1), i(B), i(n), i(1), i(1), i(64), i(16), i(1), i(1), i(0),
+                                         ctypes.c_float(1), i(0), z)
+
+    assert append(1 << 24) == -8
+    assert attention(1 << 24, 1, 0, 0) == -10 and attention(1 << 12, 1 << 12, 8, 1 << 60) == -9
+    assert attention(4, 1, 8, 100) == -12
