@@ -152,15 +152,22 @@ struct Deal {
 };
 // How a call's tiles of keys are dealt out: {0, 0}, a workgroup per problem (sequence, key head, group of rows), or workgroups to
 // deal all tiles out to and the least tiles of a part.
-//   * Up to a tile of keys there is nothing to split; 1024 sequence heads x 577 keys: 34.5 us one workgroup each, 37.7 us in
-//     parts (the join); 16 heads x 1000 keys: 9.4 and 8.3 us.
+//   * Parts cost a join, some 6 us, as long as a workgroup takes for 6 or 7 tiles of 128 keys.  So a workgroup per problem,
+//     unless parts spare each workgroup more than that: 96 heads x 1024 keys 10.1 us, in parts 12.8; 160 x 155 keys, 24 rows,
+//     9.1 and 17.9; 320 x 2048, 40 rows, 53 and 71; but 8 x 2048 keys 14.5 and 8.4, 96 x 6000 57 and 35.
+//   * Only the bound is known here.  Beyond 4096 keys lengths may differ much, which parts even out: 320 x up to 6000 keys, 20
+//     rows, 57.8 us one workgroup each, 34.5 in parts (all of one length: 136 and 147).
 //   * Otherwise as many workgroups as are resident at once by their registers, 3 per compute unit for D 128, 4 for D 64:
 //     8 x 16384 keys, 8 heads of 128: 101 us with 768, 103 with 256.
 //   * A part's (m, l, o) costs rows x D floats written and read: beyond 16 rows one workgroup per compute unit.  2 x 16384 keys,
 //     64 rows: 26.6 us with 256, 29.7 with 512; 12 ragged caches of up to 8009 keys, 40 rows: 26 and 34.
 Deal deal_out(int64_t problems, int64_t rows, int64_t bound, int64_t D) {
-  if (bound <= 128 || (problems >= 192 && bound <= 1024)) return {0, 0};
-  return {rows > 16 ? 256 : D == 64 ? 1024 : 768, 1};
+  const int64_t share = rows > 16 ? 256 : D == 64 ? 1024 : 768, resident = rows > 32 ? 256 : rows > 16 ? 512 : share;
+  if (bound <= 4096) {
+    const int64_t tiles = (bound + 127) / 128, whole = (problems + resident - 1) / resident * tiles;
+    if (whole - (problems * tiles + share - 1) / share < 7) return {0, 0};
+  }
+  return {share, 1};
 }
 
 // (q, k_pages, v_pages, table, lens, scale or None, causal, max_len or None, return_lse, share or None, least, stream)
