@@ -153,10 +153,10 @@ struct Deal {
 // How a call's tiles of keys are dealt out: {0, 0}, a workgroup per problem (sequence, key head, group of rows), or workgroups to
 // deal all tiles out to and the least tiles of a part.
 //   * Parts cost a join, some 6 us, as long as a workgroup takes for 6 or 7 tiles of 128 keys.  So a workgroup per problem,
-//     unless parts spare each workgroup more than that: 96 heads x 1024 keys 10.1 us, in parts 12.8; 160 x 155 keys, 24 rows,
-//     9.1 and 17.9; 320 x 2048, 40 rows, 53 and 71; but 8 x 2048 keys 14.5 and 8.4, 96 x 6000 57 and 35.
+//     unless parts spare each workgroup more than that: 96 heads x 1024 keys 10.1 us, in parts 12.6; 160 x 155 keys, 24 rows,
+//     9.1 and 17.9; 320 x 2048, 40 rows, 53 and 67; but 8 x 2048 keys 14.5 and 8.4, 96 x 6000 57 and 35.
 //   * Only the bound is known here.  Beyond 4096 keys lengths may differ much, which parts even out: 320 x up to 6000 keys, 20
-//     rows, 57.8 us one workgroup each, 34.5 in parts (all of one length: 136 and 147).
+//     rows, 57.4 us one workgroup each, 32.8 in parts (all of one length: 135 and 144).
 //   * Otherwise as many workgroups as are resident at once by their registers, 3 per compute unit for D 128, 4 for D 64:
 //     8 x 16384 keys, 8 heads of 128: 101 us with 768, 103 with 256.
 //   * A part's (m, l, o) costs rows x D floats written and read: beyond 16 rows one workgroup per compute unit.  2 x 16384 keys,

@@ -38,7 +38,8 @@ struct PagedAttArgs {
   const void *q, *kp, *vp;
   void* o;
   float* lse;
-  float* part;                                               // [workgroups][rows][D + 4]: o, then m, l
+  float* part;                                               // [workgroups][rows][D + 4]: o, then m, l; the first row's next
+                                                             // word: tiles of a part
   const int *table, *lens;
   long long q_bs, q_ns, q_hs;
   long long k_ps, v_ps, t_bs;                                // page strides of the cache in bytes; table rows in entries
@@ -318,15 +319,42 @@ __device__ __forceinline__ int wave_scan_i32(int v) {
   return v;
 }
 
-// How tiles are dealt out.  A problem is a sequence's key head and group of rows, H of them per sequence.  Parts have
-// max(least, all tiles / share) tiles, a problem's last one less, so there are at most share + problems of them; they are
-// numbered problem after problem.
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
+  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x111, 0xf, 0xf, false));
+  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x112, 0xf, 0xf, false));
+  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x114, 0xf, 0xf, false));
+  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x118, 0xf, 0xf, false));
+  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x142, 0xa, 0xf, false));
+  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x143, 0xc, 0xf, false));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// How tiles are dealt out.  A problem is a sequence's key head and group of rows, H of them per sequence.  Parts have `each`
+// tiles, a problem's last one less; they are numbered problem after problem.  each is at least max(least, all tiles / share), so
+// there are at most share + problems parts.  Short last parts may make them more than the `share` workgroups that are resident
+// at once, and a further round is not free: one workgroup alone takes 0.1 of the time that it takes among all of them, where
+// a row tile has few registers and the memory is the bound, 0.7 where it has many (more than 16 rows).  Then, of 64 lengths
+// from the least one to twice that, a lane each, the one that ends first by that reckoning is taken.  12 sequences x 8 heads
+// of 6000 keys, 20 rows: 86 us with the least length, 67 so; 40 x 8 heads, one row of 64: 118 and 97.
+// mine: tiles of sequence `lane`, of the first 64, 0 where there is none.
 template <int TK>
 __device__ __forceinline__ int tiles_each(const PagedAttArgs& p, int H, int lane, int mine) {
-  int sum = mine;                                            // tiles of sequence `lane`
+  int sum = mine;
   for (int b = lane + 64; b < p.B; b += 64) sum += tiles_of<TK>(p, p.lens[b]);
   const int total = __builtin_amdgcn_readlane(wave_scan_i32(sum), 63) * H;
-  return max(p.least, (total + p.share - 1) / p.share);
+  if (total <= p.share) return p.least;
+  const int least = max(p.least, (total + p.share - 1) / p.share);
+  if (p.B > 64 || p.B * H >= p.share) return least;          // more rounds than one in any case
+  if (__builtin_amdgcn_readlane(wave_scan_i32((mine + least - 1) / least), 63) * H <= p.share) return least;
+  const uint32_t each = least + lane * (1 + (least >> 6)), magic = 0xffffffffu / each + 1;      // umulhi(t, magic): t / each, or near it
+  uint32_t parts = 0;
+  for (int b = 0; b < p.B; b += 8)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) parts += __umulhi(__builtin_amdgcn_readlane(mine, b + x) + each - 1, magic);
+  const int over = (int)parts * H - p.share, few = 31 - __clz(least | 1 << 13) - 13;
+  const uint32_t more = over <= 0 ? 0 : max((uint32_t)over * 256u / (uint32_t)p.share, p.rows > 16 ? 180u : 26u);
+  const int best = (int)(wave_min_u32((each >> few) * (256u + more) << 6 | lane) & 63u);
+  return __builtin_amdgcn_readlane((int)each, best);
 }
 
 template <typename T, int D, int MT>
@@ -352,6 +380,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
     int mine = lane < p.B ? p.lens[lane] : 0;
     const int t0 = lane < p.B ? tiles_of<TK>(p, mine) : 0;
     const int each = tiles_each<TK>(p, H, lane, t0);
+    if (me == 0 && threadIdx.x == 0) reinterpret_cast<int*>(p.part)[D + 2] = each;    // for the join
     int begin = 0, src = -1, upto = 0, parts = 0;
     b = 0;
     for (; b < p.B; b += 64) {                               // the sequence of part `me`, 64 of them at a time
@@ -525,12 +554,11 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
   const int row = i * G + h - hk * G, group = row / p.rows, in = row - group * p.rows;
   const int lane = threadIdx.x & 63;
   const int own = ((const_i32)p.lens)[b];
-  const int t0 = lane < p.B ? tiles_of<TK>(p, p.lens[lane]) : 0;
-  const int each = tiles_each<TK>(p, H, lane, t0);
+  const int each = reinterpret_cast<const int*>(p.part)[D + 2];
   const int parts = (tiles_of<TK>(p, own) + each - 1) / each;
   if (parts == 1) return;                                    // written already
   int before = 0;                                            // parts of the sequences before this one
-  for (int x = lane; x < b; x += 64) before += ((x == lane ? t0 : tiles_of<TK>(p, p.lens[x])) + each - 1) / each;
+  for (int x = lane; x < b; x += 64) before += (tiles_of<TK>(p, p.lens[x]) + each - 1) / each;
   const int lo = __builtin_amdgcn_readlane(wave_scan_i32(before), 63) * H + (hk * p.groups + group) * parts;
   const int d = (threadIdx.x % TD) * 4, sl = threadIdx.x / TD;
   const float* src = p.part + (long long)in * (D + 4);
