@@ -266,27 +266,28 @@ struct Shape {
   int tiles, nw, kw, kz;                                     // tiles of 16 outputs per wave, waves over outputs and K, parts of K
 };
 
-// The share of the 256 compute units that work while `groups` equal workgroups run, and what a further part of K costs
-// besides (its sums are written and read again).
-double fill(int64_t groups, int kz) { return (double)groups * kz / ((groups * kz + 255) / 256 * 256) - 0.06 * (kz - 1); }
-
-// Few outputs (N < 8192): one tile a wave and eight waves over K, the most waves the layer can have (1 x 4096 x 1024: 3.9 us,
-// with two tiles 4.4; 16 x 4096 x 4096: 7.7 and 8.1).  Many: two tiles share a wave's x where there is one tile of rows
-// (5 x 50265 x 1024: 9.7 us, with one 11.2), four where there are more (32 x 32000 x 8192: 47.5, with two 68).
-// Where a long K leaves the last round of workgroups mostly empty, parts of K even it out: 313 workgroups in four parts
-// (20 x 20000 x 8192, groups of 64) 40.3 us, in one 48.5; 128 in two (24 x 8192 x 28672) 41.3, in one 64.7; 250 in one
-// (32 x 32000 x 8192) 47.5, in two 53.3.
+// Up to 16 rows: one tile a wave and eight waves over K as long as every workgroup has a compute unit (256 tiles: 1 x 4096 x
+// 4096 6.0 us, with two tiles 7.5), then two tiles that share a wave's x (16 x 6000 x 8192: 15 us, with one 21; 5 x 50265 x
+// 1024: 9.7 and 11.2), with fewer waves over K where there are many (30000 x 2048: 12.0 us, with eight 12.5).
+// More rows: eight tiles of products for a wave's x (four of 16 outputs, two of 16 rows) from 64 workgroups of those on
+// (200 x 4096 x 4096: 31 us, with one tile of outputs 60; 64 x 2048 x 2048: 9.5 and 7.5).  Parts of K fill compute units that
+// have nothing to do in the only or the last round of workgroups, for the price of sums written and read again, 4 / steps
+// of the work: 128 workgroups in two parts (24 x 8192 x 28672) 41.3 us, in one 64.7; 313 in four (20 x 20000 x 8192, groups of 64)
+// 40.3, in one 48.5; 188 of a shorter K in one (24 x 12000 x 4096) 18.7, in four 21.1.
 Shape shape_of(int64_t M, int64_t N, int64_t K) {
   const int steps = (int)std::min<int64_t>((K + 127) / 128, 1 << 20);
-  if (N < 8192) return {1, 1, std::min(8, steps), 1};
-  if (M <= 16) return {2, 1, std::min(4, steps), 1};
+  const int64_t tiles = (N + 15) / 16;
+  if (M <= 16) return tiles <= 256 ? Shape{1, 1, std::min(8, steps), 1} : Shape{2, 1, std::min(tiles <= 768 ? 8 : 4, steps), 1};
+  const int64_t blocks = (M + 31) / 32, wide = (tiles + 3) / 4 * blocks, groups = wide <= 64 ? tiles * blocks : wide;
+  const int kw = std::min(wide <= 64 || (steps <= 8 && wide <= 256) ? 8 : 4, steps);
+  auto worth = [&](int kz) {                                 // share of compute units, and of waves' steps, at work
+    const int part = (steps + kz - 1) / kz, turns = (part + kw - 1) / kw;
+    return (double)groups * kz / (double)((groups * kz + 255) / 256 * 256) * steps / (kz * kw * turns) - 4.0 / steps * (kz - 1);
+  };
   int kz = 1;
-  if (steps >= 64) {
-    const int64_t groups = (N + 63) / 64 * ((M + 31) / 32);
-    for (int parts = 2; parts <= 4; ++parts)
-      if (fill(groups, parts) > fill(groups, kz)) kz = parts;
-  }
-  return {4, 1, std::min(4, steps), kz};
+  for (int parts = 2; parts <= std::min(4, steps) && groups <= 384; ++parts)          // beyond, rounds overlap
+    if (worth(parts) > worth(kz)) kz = parts;
+  return {wide <= 64 ? 1 : 4, 1, kw, kz};
 }
 
 // (x, words, scale, zero, n, k, group, bias, act, res, shape or None, stream) -> y

@@ -1,6 +1,8 @@
 """The decode-step operators together (append, attention, 4-bit layers, verification), captured and on several streams, and
 in the transformer recognizer: decoders longer than 1024 positions, images of more than 1024 patches, 4-bit weights."""
 import dataclasses
+import math
+import random
 
 import pytest
 import torch
@@ -258,3 +260,22 @@ def test_recognizer_with_4_bit_weights(dev):
     again, _ = m.generate(xin, max_len=10)
     assert torch.equal(again, toks) and isinstance(m._pk["lm"][0], Q.Int4Weight)
     assert not isinstance(m.prepare(int4_group=0)._pk["lm"][0], Q.Int4Weight)
+
+
+def test_rules_give_what_the_entries_take():
+    """Launch shapes over the whole range of sizes lie within the kernels' own checks."""
+    if not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    rules, g = _loader.bind(), random.Random(0)
+    log = lambda hi: int(math.exp(g.uniform(0, math.log(hi))))  # noqa: E731
+    for _ in range(4000):
+        m, n, k = log(1 << 20), log(1 << 26), log(1 << 23)
+        tiles, nw, kw, kz = rules.rule_shape(m, n, k)
+        wide = 1 if m <= 16 else 2
+        assert tiles in (1, 2 * wide) and nw >= 1 and kw >= 1 and nw * kw <= 8 and nw * kw * tiles * wide <= 64 and 1 <= kz <= 64
+        assert kw * kz <= max(1, -(-k // 128)) * 4
+        share, least = rules.rule_deal(log(1 << 23), log(48), log(1 << 30), g.choice((64, 128)))
+        assert (share, least) == (0, 0) or (0 < share <= 1 << 20 and least >= 1)
+        b, v = log(1 << 22), log(1 << 29)
+        pieces = rules.rule_pieces(b, v)
+        assert 1 <= pieces <= 64 and (pieces == 1 or b <= 65535)
