@@ -262,3 +262,22 @@ def test_refuses_weights_of_another_layout(change, dev):
     x = torch.zeros(2, w.k, dtype=torch.bfloat16, device=w.words.device)
     with pytest.raises(ValueError):
         _loader.bind().linear_int4(x, w.words, w.scale, w.zero, w.n, w.k, w.group, None, 0, None, None, 0)
+
+
+BY_RULE = [  # rows, n, k, group, zero, res: sizes at which the rule's shapes differ, with odd ends of outputs and features
+    (24, 4203, 1024, 64, True, True), (33, 4100, 960, 64, False, False), (70, 2101, 2048, 128, True, False), (24, 1024, 4064, 32, True, True),
+    (16, 4201, 512, 32, False, True), (9, 12301, 288, 32, True, False), (200, 1030, 1152, 128, False, True), (17, 16400, 256, 128, True, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(len(BY_RULE)))
+def test_shapes_of_the_rule(i):
+    rows, n, k, group, zero, has_res = BY_RULE[i]
+    dt, sdt = (torch.float16, torch.bfloat16) if i % 2 else (torch.bfloat16, torch.float16)
+    codes, scale, z, w = layer(90 + i, n, k, group, zero, sdt)
+    g = torch.Generator().manual_seed(190 + i)
+    x = torch.randn(rows, k, generator=g).to(dt)
+    res = torch.randn(rows, n, generator=g).to(dt) if has_res else None
+    xd, rd = to("cuda", x, res)
+    check(Q.linear_int4(xd, w.to("cuda"), res=rd).cpu(), x, codes, scale, z, group, None, "none", res)
