@@ -24,7 +24,7 @@
 //
 // 100003 positions, 32 / 8 heads of 128: 82 us, 5.0 TB/s, what a copy reaches.  64 x 577 positions, 16 heads of 64: 33.8 us,
 // 4.5 TB/s.  12 x 5 tokens over ragged caches of up to 8009: 25.3 us, 2.3 TB/s; a wave has three or four tiles there, and what
-// precedes its first and follows its last one (page table, join of the waves, 6 us for the parts) is as long as their stream.
+// precedes its first and follows its last one (page table, join of the waves, 5 us for the parts) is as long as their stream.
 #include "common.h"
 #include "decode_abi.h"
 
