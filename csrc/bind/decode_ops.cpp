@@ -170,6 +170,17 @@ Deal deal_out(int64_t problems, int64_t rows, int64_t bound, int64_t D) {
   return {share, 1};
 }
 
+// The rows (new tokens x query heads) that read one key head, in groups of up to 48, three tiles of 16.  Three tiles in a wave
+// fetch a key once, but leave one workgroup per compute unit; two groups of two tiles side by side have two, which is worth
+// more while the keys are few: 8 heads x 3000 keys, 40 rows, 17.3 us as one group and 15.0 as two, 96 x 1500 33.1 and 27.3, 16 x
+// 6000 23.2 and 22.6; but 8 x 24000 32.5 and 33.8, 96 x 6000 72 and 88, 320 x 2048 with heads of 64 53 and 62.  More rows:
+// groups of up to 32 (2 x 16384 keys, 64 rows: 26.5 us, in one wave 30).
+int64_t row_groups(int64_t rows, int64_t heads, int64_t bound) {
+  if (rows <= 32) return 1;
+  if (rows > 48) return (rows + 31) / 32;
+  return (bound <= 2048 && heads < 256) || heads * ((bound + 127) / 128) <= 1000 ? 2 : 1;
+}
+
 // (q, k_pages, v_pages, table, lens, scale or None, causal, max_len or None, return_lse, share or None, least, stream)
 PyObject* attention(PyObject* const* a) {
   const at::Tensor &q = tensor(a[0]), &kp = tensor(a[1]), &vp = tensor(a[2]), &table = tensor(a[3]), &lens = tensor(a[4]);
@@ -193,7 +204,7 @@ PyObject* attention(PyObject* const* a) {
   }
   int64_t bound = width * page;
   if (a[7] != Py_None) bound = std::min<int64_t>(bound, number(a[7]));
-  const int64_t all = n * (hq / hkv), groups = all <= 48 ? 1 : (all + 31) / 32, rows = (all + groups - 1) / groups;
+  const int64_t all = n * (hq / hkv), groups = row_groups(all, B * hkv, bound), rows = (all + groups - 1) / groups;
   const int64_t problems = B * hkv * groups;
   Deal d = a[9] == Py_None ? deal_out(problems, rows, bound, D) : Deal{number(a[9]), number(a[10])};
   if (n * hq >= (int64_t)(1 << 24) / std::max<int64_t>(B, 1)) d = {0, 0};     // the join's launch ends there, and the card is full
@@ -204,7 +215,7 @@ PyObject* attention(PyObject* const* a) {
   if (d.share) part = at::empty({d.share + problems, rows, D + 4}, q.options().dtype(at::kFloat));
   launched(k_attention(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), kp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
                        vp.data_ptr(), vp.stride(0), vp.stride(1), vp.stride(2), table.data_ptr(), table.stride(0), lens.data_ptr(),
-                       o.data_ptr(), want ? lse.data_ptr() : nullptr, d.share ? part.data_ptr() : nullptr, d.share ? part.numel() : 0, as_int(d.share), as_int(d.least),
+                       o.data_ptr(), want ? lse.data_ptr() : nullptr, d.share ? part.data_ptr() : nullptr, d.share ? part.numel() : 0, as_int(groups), as_int(d.share), as_int(d.least),
                        as_int(B), as_int(n), as_int(hq), as_int(hkv), as_int(D), as_int(page), as_int(width), as_int(kp.size(0)), truth(a[6]),
                        (float)scale, half_type(q.scalar_type()), w.stream),
            "dlamd_paged_attention");
@@ -272,8 +283,8 @@ struct Shape {
 // More rows: eight tiles of products for a wave's x (four of 16 outputs, two of 16 rows) from 64 workgroups of those on
 // (200 x 4096 x 4096: 31 us, with one tile of outputs 60; 64 x 2048 x 2048: 9.5 and 7.5).  Parts of K fill compute units that
 // have nothing to do in the only or the last round of workgroups, for the price of sums written and read again, 4 / steps
-// of the work: 128 workgroups in two parts (24 x 8192 x 28672) 41.3 us, in one 64.7; 313 in four (20 x 20000 x 8192, groups of 64)
-// 40.3, in one 48.5; 188 of a shorter K in one (24 x 12000 x 4096) 18.7, in four 21.1.
+// of the work: 128 workgroups in two parts (24 x 8192 x 28672) 41.3 us, in one 64.7; 313 in four (20 x 20000 x 8192, groups of
+// 64) 40.3, in one 48.5; 188 of a shorter K in one (24 x 12000 x 4096) 18.7, in four 21.1.
 Shape shape_of(int64_t M, int64_t N, int64_t K) {
   const int steps = (int)std::min<int64_t>((K + 127) / 128, 1 << 20);
   const int64_t tiles = (N + 15) / 16;

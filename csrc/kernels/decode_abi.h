@@ -14,7 +14,7 @@ int dlamd_paged_append(const void* k, long long k_ts, long long k_hs, const void
 int dlamd_paged_attention(const void* q, long long q_bs, long long q_ns, long long q_hs, const void* kp, long long kp_ps,
                           long long kp_ss, long long kp_hs, const void* vp, long long vp_ps, long long vp_ss, long long vp_hs,
                           const void* table, long long t_bs, const void* lens, void* o, void* lse, void* part, long long part_floats,
-                          int share, int least, int B, int n, int Hq, int Hkv, int D, int page, int width, int pages, int causal,
+                          int groups, int share, int least, int B, int n, int Hq, int Hkv, int D, int page, int width, int pages, int causal,
                           float scale, int dtype, ihipStream_t* stream);
 int dlamd_verify_draft(const void* draft, long long d_bs, const void* p, long long p_bs, long long p_ns, const void* q, long long q_bs,
                        long long q_ns, const void* u, long long u_bs, const void* counts, void* tokens, void* accepted, void* sums,

@@ -7,7 +7,8 @@
 //
 // The cost is reading the cache once, so everything serves loads in flight:
 //   * The n new tokens x (heads / kv_heads) query heads that read one key head are the rows of ONE problem (up to 48 per
-//     workgroup): a key is fetched once for all of them and the products run on matrix instructions, padded to 16.
+//     workgroup, further groups on the same die): a key is fetched once for all of them and the products run on matrix
+//     instructions, padded to 16.
 //   * A wave takes tiles of 32 keys by itself, straight from memory into the operand registers, the next tile's loads in
 //     flight while it computes; no LDS, no barrier until the four waves of a workgroup join their (m, l, o).
 //   * S^T = K Q^T: A = K (a lane holds 8 dimensions of one key, as they lie in memory), so a lane's accumulators are 4 keys
@@ -357,6 +358,13 @@ __device__ __forceinline__ int tiles_each(const PagedAttArgs& p, int H, int lane
   return __builtin_amdgcn_readlane((int)each, best);
 }
 
+// Workgroups go to the 8 dies of the card in turn, each with an L2 cache of its own: groups of rows that read the same keys are
+// 8 apart, so that one fetch from memory serves them.  A permutation of the launch; its last, incomplete stretch stays.
+__device__ __forceinline__ int neighbours(int at, int groups, int grid) {
+  const int stretch = 8 * groups, first = at / stretch * stretch, in = at - first;
+  return groups == 1 || first + stretch > grid ? at : first + (in & 7) * groups + (in >> 3);
+}
+
 template <typename T, int D, int MT>
 __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_attention_kernel(const PagedAttArgs p) {
   typedef typename Mat<T>::x8 x8;
@@ -366,14 +374,14 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int G = p.Hq / p.Hkv, R = p.n * G, H = p.Hkv * p.groups;
-  const int cap = p.width * p.page, me = blockIdx.x;
+  const int cap = p.width * p.page, me = neighbours(blockIdx.x, p.groups, gridDim.x);
 
   // which problem and which of its tiles
   int b, head, kept, tile = 0, tiles = 0x7fffffff;
   bool whole = true;
   if (p.share == 0) {
     b = me / H;
-    head = me - b * H;
+    head = me - b * H;                                       // groups of one key head side by side
     b = __builtin_amdgcn_readfirstlane(b);
     kept = ((const_i32)p.lens)[b];
   } else {
@@ -400,8 +408,10 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
     kept = __builtin_amdgcn_readlane(mine, src);
     parts = __builtin_amdgcn_readlane(parts, src);
     const int in = me - (__builtin_amdgcn_readlane(upto, src) - parts * H);
-    head = in / parts;
-    tile = (in - head * parts) * each;
+    const int unit = in / p.groups;                          // key head after key head, part after part, group after group
+    const int h = unit / parts;
+    head = h * p.groups + in - unit * p.groups;
+    tile = (unit - h * parts) * each;
     tiles = each;
     whole = parts == 1;
   }
@@ -559,14 +569,14 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
   if (parts == 1) return;                                    // written already
   int before = 0;                                            // parts of the sequences before this one
   for (int x = lane; x < b; x += 64) before += (tiles_of<TK>(p, p.lens[x]) + each - 1) / each;
-  const int lo = __builtin_amdgcn_readlane(wave_scan_i32(before), 63) * H + (hk * p.groups + group) * parts;
+  const int lo = __builtin_amdgcn_readlane(wave_scan_i32(before), 63) * H + hk * parts * p.groups + group;
   const int d = (threadIdx.x % TD) * 4, sl = threadIdx.x / TD;
   const float* src = p.part + (long long)in * (D + 4);
   float m = ROW_NONE, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = lo + sl; s < lo + parts; s += SL) {
-    const float* q = src + (long long)s * p.rows * (D + 4);
+  for (int s = sl; s < parts; s += SL) {
+    const float* q = src + (long long)(lo + s * p.groups) * p.rows * (D + 4);
     const float ms = q[D], ls = q[D + 1], mn = fmaxf(m, ms);
     const f32x4 os = *reinterpret_cast<const f32x4*>(q + d);
     const float a = __builtin_amdgcn_exp2f(m - mn), c = __builtin_amdgcn_exp2f(ms - mn);
@@ -611,13 +621,14 @@ static void launch_rows(const PagedAttArgs& a, int rows, hipStream_t stream) {
 }
 
 // q: [B, n, Hq, D] (strides given), o: [B, n, Hq, D] contiguous, lse: [B, n, Hq] or null.  dtype: 0 bf16, 1 fp16.
+// groups: the n x Hq / Hkv rows that read one key head in so many groups, of at most 48.
 // share: 0 (a workgroup per sequence, key head and group of rows) or workgroups to deal all tiles out to, in parts of at least
 // `least` tiles; part: [share + problems][rows of a problem][D + 4] floats where share > 0.
 extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_ns, long long q_hs, const void* kp,
                                      long long kp_ps, long long kp_ss, long long kp_hs, const void* vp, long long vp_ps,
                                      long long vp_ss, long long vp_hs, const void* table, long long t_bs,
                                      const void* lens, void* o, void* lse, void* part, long long part_floats,
-                                     int share, int least, int B, int n,
+                                     int groups, int share, int least, int B, int n,
                                      int Hq, int Hkv, int D, int page, int width, int pages, int causal, float scale,
                                      int dtype, hipStream_t stream) {
   if (B <= 0 || n <= 0 || Hq <= 0) return 0;
@@ -635,10 +646,9 @@ extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_
   if (dtype != 0 && dtype != 1) return -6;
   if (share < 0 || share > (1 << 20) || (share > 0 && (least < 1 || !part || ((uintptr_t)part & 15)))) return -7;
   if ((long long)n * Hq > 0x7fffffffLL || (share > 0 && (long long)n * Hq >= (1LL << 24) / B)) return -9;   // the join: a workgroup per row
-  // Rows of one problem, in tiles of 16.  Up to 48 share a key's fetch (12 ragged caches, 40 rows: 26 us; as two groups that
-  // fetch it twice 31); beyond, groups of up to 32 (64 rows in one wave: 30 us for 2 x 16384 keys, in two groups 26.5: the
-  // registers of more rows leave one workgroup per compute unit).
-  const int R = n * (Hq / Hkv), groups = R <= 48 ? 1 : (R + 31) / 32, rows = (R + groups - 1) / groups;
+  const int R = n * (Hq / Hkv);
+  if (groups < 1 || groups > R || (R + groups - 1) / groups > 48) return -8;
+  const int rows = (R + groups - 1) / groups;
   if (share > 0 && part_floats < ((long long)share + (long long)B * Hkv * groups) * rows * (D + 4)) return -12;
   // problems, parts and tiles are counted in 32 bits, the launch in 2^24 workgroups
   if ((long long)B * Hkv * groups + share >= (1LL << 24)) return -10;

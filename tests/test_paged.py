@@ -602,9 +602,24 @@ def test_c_entries_refuse_more_than_a_launch_holds():
 
     def attention(B, n, share, floats):
         return lib.dlamd_paged_attention(at, ll(64), ll(64), ll(64), at, ll(1024), ll(64), ll(64), at, ll(1024), ll(64), ll(64), at, ll(1),
-                                         at, at, z, at, ll(floats), i(share), i(1), i(B), i(n), i(1), i(1), i(64), i(16), i(1), i(1), i(0),
+                                         at, at, z, at, ll(floats), i(1), i(share), i(1), i(B), i(n), i(1), i(1), i(64), i(16), i(1), i(1), i(0),
                                          ctypes.c_float(1), i(0), z)
 
     assert append(1 << 24) == -8
     assert attention(1 << 24, 1, 0, 0) == -10 and attention(1 << 12, 1 << 12, 8, 1 << 60) == -9
     assert attention(4, 1, 8, 100) == -12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("share,least", [(None, 0), (0, 0), (1, 1), (37, 1), (256, 1), (256, 9)])
+@pytest.mark.parametrize("n,hq,hkv,D,dt", [(5, 16, 2, 128, "fp16"), (5, 16, 2, 64, "bf16"), (3, 30, 2, 128, "bf16"), (11, 8, 2, 64, "fp16")])
+def test_attention_kernel_with_three_tiles_of_rows(n, hq, hkv, D, dt, share, least, monkeypatch):
+    """33 to 48 rows stay together where the cache may be long: a wide table that is mostly empty.  A tight bound splits them,
+    and the result is right either way."""
+    monkeypatch.setattr(P, "_DEAL", (share, least))
+    c = att_case(31, [400, 0, -1, 47, 1, 300, 129, 128], n, 16, hq, hkv, D, DTYPES[dt], True)
+    c["table"] = torch.cat((c["table"], torch.full((8, 1024), -1, dtype=torch.int32)), 1)
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    for bound in (None, 500):
+        o, lse = P.paged_attention(**d, return_lse=True, max_len=bound)
+        check_attention(c, o.cpu(), lse.cpu())
