@@ -61,6 +61,14 @@ __device__ __forceinline__ int dlamd_xcd_remap(int bid, int nwg) {
   return start + idx;
 }
 
+// The other way round: of every 8 x `each` consecutive workgroups, the `each` that read the same data get
+// consecutive logical ids and sit 8 apart, on one XCD at one time, while all XCDs stay equally full
+// however many logical ids at the end are unused.  A permutation; the last, incomplete stretch stays.
+__device__ __forceinline__ int dlamd_xcd_neighbours(int bid, int each, int nwg) {
+  const int stretch = DLAMD_NUM_XCD * each, first = bid / stretch * stretch, in = bid - first;
+  return each == 1 || first + stretch > nwg ? bid : first + in % DLAMD_NUM_XCD * each + in / DLAMD_NUM_XCD;
+}
+
 __device__ __forceinline__ float wave_reduce_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
