@@ -53,7 +53,8 @@ struct PagedAttArgs {
   uint32_t flip;                                             // sign bits to turn in q where the scale is negative
 };
 
-#define ROW_NONE (-3.4028234e38f)                            // running maximum of nothing: finite, so differences stay numbers
+#define ROW_NONE (-3.4028234e38f)                            // running maximum (of unscaled scores) of nothing: finite, so differences
+                                                             // stay numbers
 #define LN2 0.6931471805599453f
 
 // mul: a 16x16x32 product; split: two weights as 16-bit halves hi + lo (hi may be rounded either way, lo makes up for it).
@@ -177,7 +178,8 @@ __device__ __forceinline__ void scores(f32x4 (&x)[MT][2], const Rows<T, D, MT>& 
   }
 }
 
-// Scores to weights, against the running maximum (which is kept scaled, in units of log 2).
+// Scores to weights, against the running maximum.  Scores are scaled behind the difference: a maximum that is itself scaled
+// and rounded is off by half a step of its own, which from scores of 2^31 on is more than the exponential's range.
 template <typename T, int D, int MT>
 __device__ __forceinline__ void weights(typename Mat<T>::x8 (&hi)[MT], typename Mat<T>::x8 (&lo)[MT], Rows<T, D, MT>& w,
                                         const f32x4 (&x)[MT][2], float scale2) {
@@ -186,12 +188,11 @@ __device__ __forceinline__ void weights(typename Mat<T>::x8 (&hi)[MT], typename 
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(x[mt][0][j], x[mt][1][j]));
-    top *= scale2;
     if (__any(top > w.m[mt])) {                              // rare once the largest scores have been seen
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float m = fmaxf(w.m[mt], top);
-      const float a = __builtin_amdgcn_exp2f(w.m[mt] - m);
+      const float a = __builtin_amdgcn_exp2f((w.m[mt] - m) * scale2);
       w.m[mt] = m;
       w.l[mt] *= a;
 #pragma unroll
@@ -204,8 +205,8 @@ __device__ __forceinline__ void weights(typename Mat<T>::x8 (&hi)[MT], typename 
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int h = c >> 1, j = 2 * (c & 1);
-      const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[mt][h][j], scale2, -w.m[mt]));
-      const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[mt][h][j + 1], scale2, -w.m[mt]));
+      const float e0 = __builtin_amdgcn_exp2f((x[mt][h][j] - w.m[mt]) * scale2);
+      const float e1 = __builtin_amdgcn_exp2f((x[mt][h][j + 1] - w.m[mt]) * scale2);
       sum += e0 + e1;
       uint32_t a, b;
       Mat<T>::split(e0, e1, a, b);
@@ -289,7 +290,7 @@ __device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedA
 #pragma unroll
           for (int j = 0; j < 8; ++j) x += (float)a[j] * (float)c[j];
         }
-        const float e = __builtin_amdgcn_exp2f((p.flip ? -x : x) * p.scale2 - w.m[mt]);
+        const float e = __builtin_amdgcn_exp2f(((p.flip ? -x : x) - w.m[mt]) * p.scale2);
 #pragma unroll
         for (int d = 0; d < D / 4; d += 8) {                 // the lane's sums: dimensions D / 4 g .. of its query
           const x8 v = *reinterpret_cast<const x8*>(vr + d);
@@ -512,7 +513,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
       float f[4], sum = 0.f;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        f[x] = __builtin_amdgcn_exp2f(s_m[x][rr] - m);
+        f[x] = __builtin_amdgcn_exp2f((s_m[x][rr] - m) * p.scale2);
         sum += f[x] * s_l[x][rr];
       }
       float o[D / 16];
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
         T* dst = (T*)p.o + to * D + d0;
 #pragma unroll
         for (int d = 0; d < D / 16; d += 4) *reinterpret_cast<u32x2*>(dst + d) = *reinterpret_cast<u32x2*>(t + d);
-        if (p.lse && d0 == 0) p.lse[to] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * LN2;
+        if (p.lse && d0 == 0) p.lse[to] = sum == 0.f ? -INFINITY : (m * p.scale2 + __log2f(sum)) * LN2;
       } else {
         float* dst = part + in * (D + 4);
 #pragma unroll
@@ -574,7 +575,7 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
     const float* q = src + (long long)(lo + s * p.groups) * p.rows * (D + 4);
     const float ms = q[D], ls = q[D + 1], mn = fmaxf(m, ms);
     const f32x4 os = *reinterpret_cast<const f32x4*>(q + d);
-    const float a = __builtin_amdgcn_exp2f(m - mn), c = __builtin_amdgcn_exp2f(ms - mn);
+    const float a = __builtin_amdgcn_exp2f((m - mn) * p.scale2), c = __builtin_amdgcn_exp2f((ms - mn) * p.scale2);
     l = l * a + ls * c;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = o[j] * a + os[j] * c;
@@ -592,12 +593,12 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
     for (int x = 0; x < SL; ++x) top = fmaxf(top, s_m[x]);
 #pragma unroll
     for (int x = 0; x < SL; ++x) {
-      const float f = __builtin_amdgcn_exp2f(s_m[x] - top);
+      const float f = __builtin_amdgcn_exp2f((s_m[x] - top) * p.scale2);
       sum2 += f * s_l[x];
       v += f * s_o[x][threadIdx.x];
     }
     ((T*)p.o)[to * D + threadIdx.x] = (T)(sum2 == 0.f ? 0.f : v / sum2);
-    if (p.lse && threadIdx.x == 0) p.lse[to] = sum2 == 0.f ? -INFINITY : (top + __log2f(sum2)) * LN2;
+    if (p.lse && threadIdx.x == 0) p.lse[to] = sum2 == 0.f ? -INFINITY : (top * p.scale2 + __log2f(sum2)) * LN2;
   }
 }
 

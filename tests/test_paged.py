@@ -623,3 +623,40 @@ def test_attention_kernel_with_three_tiles_of_rows(n, hq, hkv, D, dt, share, lea
     for bound in (None, 500):
         o, lse = P.paged_attention(**d, return_lse=True, max_len=bound)
         check_attention(c, o.cpu(), lse.cpu())
+
+
+# ---------------------------------------------------------------------------------------------- weights over their whole range
+def far_case(size, sign, dt, seed=0):
+    """Scores around sign * size: keys are multiples of the signs of q, one of them a seventh or more above all others."""
+    g = torch.Generator().manual_seed(seed)
+    B, hkv, G, D, page, kept = 24, 2, 3, 64, 16, 300
+    table, pages = tables([kept] * B, page, g)
+    vp = torch.randn(pages, page, hkv, D, generator=g).to(dt)
+    signs = torch.randint(0, 2, (B, hkv, D), generator=g) * 2.0 - 1.0
+    level = (size * 8 / D) ** 0.5                                # scale is 1 / 8
+    q = signs[:, :, None] * level * (1 + torch.randint(0, 16, (B, hkv, G, 1), generator=g) / 16)
+    kp = torch.zeros(pages, page, hkv, D)
+    for b in range(B):
+        steps = 1 + torch.randint(16, 48, (kept,), generator=g) / 64
+        steps[int(torch.randint(0, kept, (1,), generator=g))] = 1 + 63 / 64 if sign > 0 else 1.0
+        for p in range(kept):
+            kp[int(table[b, p // page]), p % page] = sign * signs[b] * level * steps[p]
+    return dict(q=q.reshape(B, 1, hkv * G, D).to(dt), k_pages=kp.to(dt), v_pages=vp, table=table,
+                lens=torch.full((B,), kept, dtype=torch.int32), causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dt,size", [("bf16", 2.0 ** e) for e in (12, 24, 28, 32, 36, 60, 100)] + [("fp16", 2.0 ** e) for e in (12, 24, 28, 31)])
+@pytest.mark.parametrize("share", [0, 64])
+def test_attention_kernel_with_far_scores(dt, size, sign, share, monkeypatch):
+    """The largest score is hundreds above the next, so one key is the result: its value (a product with its weight and a
+    division by it: two fp32 roundings).  The log-sum-exp is that score: D + 4 roundings of 2^-24."""
+    monkeypatch.setattr(P, "_DEAL", (share, 1))
+    c = far_case(size, sign, DTYPES[dt])
+    ref, ref_lse = P.paged_attention_reference(**c, dtype=torch.float64)
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o, lse = (x.cpu() for x in P.paged_attention(**d, return_lse=True))
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    assert bool(((o.double() - ref).abs() <= 2.0 ** -20 * ref.abs()).all())
+    assert bool(((lse.double() - ref_lse).abs() <= 2.0 ** -24 * 68 * ref_lse.abs()).all())
