@@ -17,7 +17,9 @@
 //     dimensions of its 8 keys (16 lanes cover a key's row: whole lines) and turns the block in registers; output tile i
 //     then holds dimension (D / 16) r + i in row r, which leaves a lane with D / 4 consecutive dimensions of one query.
 //   * P goes into the products as two 16-bit halves, hi + lo: one rounding to 16 bits would cost as much accuracy as the
-//     result's own rounding, and the second product hides behind the loads.
+//     result's own rounding, and the second product hides behind the loads.  bf16 halves keep 16 bits of every weight.  fp16
+//     ends at 2^-24, so weights (and l, and o) are 2^14 times as large there: 22 bits down to 2^-18 of the largest weight,
+//     and nothing above 2^-38 of it is lost (unshifted, truncation took 3 % of weights of e^-14 of the largest).
 //   * Long caches are cut into parts of as many tiles (of 128 keys) as give every compute unit its share.  The size of a
 //     part is computed on the device from the lengths of the whole batch, so neither one long sequence nor a batch of very
 //     different lengths leaves compute units idle, and a captured call adapts while lengths grow.  A part is written as
@@ -57,9 +59,11 @@ struct PagedAttArgs {
                                                              // stay numbers
 #define LN2 0.6931471805599453f
 
-// mul: a 16x16x32 product; split: two weights as 16-bit halves hi + lo (hi may be rounded either way, lo makes up for it).
+// mul: a 16x16x32 product; split: two weights as 16-bit halves hi + lo (hi may be rounded either way, lo makes up for it); UP:
+// weights are 2^UP exp(score - maximum).
 template <typename T> struct Mat;
 template <> struct Mat<bf16_t> {
+  static constexpr float UP = 0.f;
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
   typedef __bf16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -71,6 +75,7 @@ template <> struct Mat<bf16_t> {
   static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mat<f16_t> {
+  static constexpr float UP = 14.f;
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
@@ -205,8 +210,8 @@ __device__ __forceinline__ void weights(typename Mat<T>::x8 (&hi)[MT], typename 
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int h = c >> 1, j = 2 * (c & 1);
-      const float e0 = __builtin_amdgcn_exp2f((x[mt][h][j] - w.m[mt]) * scale2);
-      const float e1 = __builtin_amdgcn_exp2f((x[mt][h][j + 1] - w.m[mt]) * scale2);
+      const float e0 = __builtin_amdgcn_exp2f((x[mt][h][j] - w.m[mt]) * scale2 + Mat<T>::UP);
+      const float e1 = __builtin_amdgcn_exp2f((x[mt][h][j + 1] - w.m[mt]) * scale2 + Mat<T>::UP);
       sum += e0 + e1;
       uint32_t a, b;
       Mat<T>::split(e0, e1, a, b);
@@ -290,7 +295,7 @@ __device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedA
 #pragma unroll
           for (int j = 0; j < 8; ++j) x += (float)a[j] * (float)c[j];
         }
-        const float e = __builtin_amdgcn_exp2f(((p.flip ? -x : x) - w.m[mt]) * p.scale2);
+        const float e = __builtin_amdgcn_exp2f(((p.flip ? -x : x) - w.m[mt]) * p.scale2 + Mat<T>::UP);
 #pragma unroll
         for (int d = 0; d < D / 4; d += 8) {                 // the lane's sums: dimensions D / 4 g .. of its query
           const x8 v = *reinterpret_cast<const x8*>(vr + d);
@@ -533,7 +538,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
         T* dst = (T*)p.o + to * D + d0;
 #pragma unroll
         for (int d = 0; d < D / 16; d += 4) *reinterpret_cast<u32x2*>(dst + d) = *reinterpret_cast<u32x2*>(t + d);
-        if (p.lse && d0 == 0) p.lse[to] = sum == 0.f ? -INFINITY : (m * p.scale2 + __log2f(sum)) * LN2;
+        if (p.lse && d0 == 0) p.lse[to] = sum == 0.f ? -INFINITY : (m * p.scale2 + (__log2f(sum) - Mat<T>::UP)) * LN2;
       } else {
         float* dst = part + in * (D + 4);
 #pragma unroll
@@ -598,7 +603,7 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
       v += f * s_o[x][threadIdx.x];
     }
     ((T*)p.o)[to * D + threadIdx.x] = (T)(sum2 == 0.f ? 0.f : v / sum2);
-    if (p.lse && threadIdx.x == 0) p.lse[to] = sum2 == 0.f ? -INFINITY : (top * p.scale2 + __log2f(sum2)) * LN2;
+    if (p.lse && threadIdx.x == 0) p.lse[to] = sum2 == 0.f ? -INFINITY : (top * p.scale2 + (__log2f(sum2) - Mat<T>::UP)) * LN2;
   }
 }
 

@@ -660,3 +660,42 @@ def test_attention_kernel_with_far_scores(dt, size, sign, share, monkeypatch):
     assert torch.isfinite(o).all() and torch.isfinite(lse).all()
     assert bool(((o.double() - ref).abs() <= 2.0 ** -20 * ref.abs()).all())
     assert bool(((lse.double() - ref_lse).abs() <= 2.0 ** -24 * 68 * ref_lse.abs()).all())
+
+
+def sink_case(gap, kept, dt, D, at):
+    """One key `gap` nats above all others, with a value of zero: the result is what the small weights add up to.  q is all
+    ones and the sink's key all gap / D, so its score is exact; the others' scores lie within a few tenths of zero, their
+    values between 0.5 and 1.5."""
+    g = torch.Generator().manual_seed(gap * 1000 + kept)
+    page, hkv, G = 16, 2, 2
+    table, pages = tables([kept] * 2, page, g)
+    kp = (torch.randn(pages, page, hkv, D, generator=g) * 0.02).to(dt)
+    vp = (torch.rand(pages, page, hkv, D, generator=g) + 0.5).to(dt)
+    for b in range(2):
+        pos = (at, kept - 1 - at)[b]
+        kp[int(table[b, pos // page]), pos % page] = gap / D
+        vp[int(table[b, pos // page]), pos % page] = 0.0
+    return dict(q=torch.ones(2, 1, hkv * G, D, dtype=dt), k_pages=kp, v_pages=vp, table=table,
+                lens=torch.full((2,), kept, dtype=torch.int32), causal=False, scale=1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("gap,kept,D,at", [(10, 200, 64, 3), (12, 4096, 128, 1000), (14, 32, 64, 7), (14, 4096, 64, 2048), (16, 32, 128, 0),
+                                           (16, 20000, 64, 17), (20, 4096, 64, 4095), (24, 20000, 128, 9999)])
+@pytest.mark.parametrize("share", [0, 64, None])
+def test_attention_kernel_keeps_small_weights(gap, kept, D, at, dt, share, monkeypatch):
+    """Tolerance: half a step of the result, and relative to sum p |v| (the result itself: values are positive): the sink's score
+    and a key's are each off by (D + 2) 2^-24 of the sum of |q k| (gap, and less than 2.5), the split of a weight into
+    two numbers of 16 bits by 2^-16, the fp32 sums and the exponential by 2^-18."""
+    if share is not None:
+        monkeypatch.setattr(P, "_DEAL", (share, 1))
+    c = sink_case(gap, kept, DTYPES[dt], D, at)
+    ref, ref_lse = P.paged_attention_reference(**c, dtype=torch.float64)
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o, lse = (x.cpu().double() for x in P.paged_attention(**d, return_lse=True))
+    weight = 2.0 ** -24 * (D + 2) * (gap + 2.5) + 2.0 ** -16 + 2.0 ** -18
+    step = torch.finfo(DTYPES[dt]).eps / 2 * ref.abs() + (2.0 ** -25 if dt == "fp16" else 0.0)       # fp16's last step is 2^-24
+    err, tol = (o - ref).abs(), step + weight * ref.abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+    assert bool(((lse - ref_lse).abs() <= 2.0 ** -24 * (D + 8) * (gap + 2.5)).all())
