@@ -263,17 +263,21 @@ __device__ __forceinline__ void add_values(Rows<T, D, MT>& w, uint32_t (&v)[8][D
   }
 }
 
-// The wave's sums of values once more, element by element, for data the products above do not serve: a value that is no
+// The wave's m, l and o once more, element by element, for data the products above do not serve: a value that is no
 // finite number at a position that some rows see and others do not (0 x NaN), or an infinite one (hi and lo weights of both
-// signs).  m and l stand.
+// signs).  Scores are summed in another order here, and where they are large that moves a weight by more than a rounding, so
+// maximum and sum are taken from these scores too.
 template <typename T, int D, int MT, int TK>
 __device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedAttArgs& p, const_i32 row, int b, int hk, int row0,
                                                  int R, int G, int first, int limit, int r, int g) {
   typedef typename Mat<T>::x8 x8;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < MT; ++mt) {
+    w.m[mt] = ROW_NONE;
+    w.l[mt] = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) w.o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 #pragma unroll 1
   for (int k0 = first; k0 < limit; k0 += TK) {
 #pragma unroll 1
@@ -295,7 +299,18 @@ __device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedA
 #pragma unroll
           for (int j = 0; j < 8; ++j) x += (float)a[j] * (float)c[j];
         }
-        const float e = __builtin_amdgcn_exp2f(((p.flip ? -x : x) - w.m[mt]) * p.scale2 + Mat<T>::UP);
+        x = p.flip ? -x : x;
+        if (x > w.m[mt]) {
+          const float a = __builtin_amdgcn_exp2f((w.m[mt] - x) * p.scale2);
+          w.m[mt] = x;
+          w.l[mt] *= a;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w.o[mt][i][j] *= a;
+        }
+        const float e = __builtin_amdgcn_exp2f((x - w.m[mt]) * p.scale2 + Mat<T>::UP);
+        if (g == 0) w.l[mt] += e;                            // the lane groups' sums are added up; here each has all keys
 #pragma unroll
         for (int d = 0; d < D / 4; d += 8) {                 // the lane's sums: dimensions D / 4 g .. of its query
           const x8 v = *reinterpret_cast<const x8*>(vr + d);

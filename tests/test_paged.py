@@ -699,3 +699,28 @@ def test_attention_kernel_keeps_small_weights(gap, kept, D, at, dt, share, monke
     err, tol = (o - ref).abs(), step + weight * ref.abs()
     assert bool((err <= tol).all()), float((err / tol).max())
     assert bool(((lse - ref_lse).abs() <= 2.0 ** -24 * (D + 8) * (gap + 2.5)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("share", [0, 64])
+def test_attention_kernel_with_an_odd_value_and_large_scores(dt, share, monkeypatch):
+    """NaN in one dimension of one visible value leaves the others alone, also where scores are large: a rounding of theirs is
+    then no small part of a weight, and weights and their sum have to come from the same scores.  One key stands out, so the
+    other dimensions are its value's."""
+    monkeypatch.setattr(P, "_DEAL", (share, 1))
+    dtype, g = DTYPES[dt], torch.Generator().manual_seed(3)
+    c = att_case(21, [90, 200, 33, 64], 1, 16, 8, 2, 64, dtype, False)
+    c["q"] = (torch.randn(4, 1, 8, 64, generator=g) * 100).to(dtype)
+    for h in range(2):
+        c["q"][:, :, 4 * h : 4 * h + 4] = c["q"][:, :, 4 * h : 4 * h + 1]      # the rows of a key head alike: one key for all
+    for b, pos in enumerate((40, 3, 32, 63)):
+        pid = int(c["table"][b, pos // 16])
+        c["k_pages"][pid, pos % 16] = c["q"][b, 0].view(2, 4, 64)[:, 0]
+        c["v_pages"][pid, pos % 16, :, 9] = float("nan")
+    ref, _ = P.paged_attention_reference(**c, dtype=torch.float64)
+    d = {x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}
+    o = P.paged_attention(**d).cpu()
+    dims = [i for i in range(64) if i != 9]
+    assert torch.isnan(o[..., 9]).all() and torch.isnan(ref[..., 9]).all()
+    assert bool(((o.double() - ref)[..., dims].abs() <= 2.0 ** -20 * ref[..., dims].abs()).all())
