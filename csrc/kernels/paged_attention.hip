@@ -499,12 +499,16 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
     weights<T, D, MT>(hi, lo, w, x, p.scale2);
     add_values<T, D, MT, true>(w, v, hi, lo, pl, k0, limit_all, limit, g, odd);
   }
+  // Only rows that are written count: a row of zeros that fills a tile up is NaN from any key with an infinite component.
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < MT; ++mt) {
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) odd |= w.o[mt][i][j] != w.o[mt][i][j];
+      for (int j = 0; j < 4; ++j) nan |= w.o[mt][i][j] != w.o[mt][i][j];
+    odd |= nan && r < min(p.rows, R - row0) - 16 * mt;
+  }
   if (__any(odd)) add_values_again<T, D, MT, TK>(w, p, row, b, hk, row0, R, G, kb + 32 * wave, limit, r, g);
   float* part = p.part + (long long)me * p.rows * (D + 4);
   // join the four waves, 16 rows at a time

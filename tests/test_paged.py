@@ -724,3 +724,19 @@ def test_attention_kernel_with_an_odd_value_and_large_scores(dt, share, monkeypa
     dims = [i for i in range(64) if i != 9]
     assert torch.isnan(o[..., 9]).all() and torch.isnan(ref[..., 9]).all()
     assert bool(((o.double() - ref)[..., dims].abs() <= 2.0 ** -20 * ref[..., dims].abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("n,D", [(1, 64), (3, 128)])
+def test_a_key_with_an_infinite_component_weighs_nothing(n, D, dt):
+    """Its score is -inf for every row; one that is merely far below gives the same bits (no row is summed in another way)."""
+    c = att_case(17, [300, 77, 128, 500], n, 16, 8, 4, D, DTYPES[dt], True)
+    c["q"] = (c["q"].abs() + 0.1).to(DTYPES[dt])
+    out = []
+    for low in (-math.inf, -3e4):
+        for b, pos in enumerate((20, 70, 127, 450)):
+            c["k_pages"][int(c["table"][b, pos // 16]), pos % 16, :, 5] = low
+        out.append(P.paged_attention(**{x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}, return_lse=True))
+    assert torch.isfinite(out[0][0]).all() and torch.equal(out[0][1], out[1][1])
+    assert torch.equal(out[0][0].view(torch.int16), out[1][0].view(torch.int16))
