@@ -11,7 +11,9 @@
 // The offset leaves again after each group of G features,
 //     sum x (c - z) = sum x (off + c) - (off + z) sum x,
 // where sum x comes from one more matrix instruction (its other operand is all ones), so scale and zero cost one fused
-// multiply-add per group and output, not one per weight.  All sums are fp32.
+// multiply-add per group and output, not one per weight.  All sums are fp32.  An infinity in x would make that difference
+// NaN, and so would bf16 values near the end of their range, whose sums with the offset overflow: an output that is no
+// finite number is summed once more without the offset (plain4).
 //
 // The waves of a workgroup share R tiles of 16 outputs and split K between them, 128 features at a time; their sums meet in
 // LDS.  The next step's loads are in flight while a step is computed.
@@ -34,7 +36,7 @@ struct Int4Args {
   void* y;
   long long x_rs, res_rs;
   float* part;                                               // [kz][M][N rounded up to 16] sums of the parts of K
-  int M, N, K, act, kw, kz, z_on;                            // z_on: 1, or 0 where `zero` is one word of eights
+  int M, N, K, G, act, kw, kz, z_on;                         // z_on: 1, or 0 where `zero` is one word of eights
 };
 
 template <typename T> struct Mat4;
@@ -155,6 +157,33 @@ __device__ __forceinline__ void use_step(f32x4 (&y)[R][CT], const u32x4 (&words)
   }
 }
 
+// Four consecutive sums as they are if they are finite; the others once more, weight by weight.
+template <typename T, typename S>
+__device__ __forceinline__ f32x4 plain4(const Int4Args& a, f32x4 v, int m, int n) {
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) odd |= !(fabsf(v[j]) < INFINITY);
+  if (!odd) return v;
+  const int tiles = (a.N + 15) >> 4, Ks = (a.K + 127) >> 7;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int k = 0; k < a.K; k += 8) {
+    const auto x = *reinterpret_cast<const typename Mat4<T>::x8*>((const T*)a.x + m * a.x_rs + k);
+    const long long at = (long long)(k / a.G) * (tiles * 16) + n;
+    const uint32_t* words = a.w + (((long long)(n >> 4) * Ks + (k >> 7)) * 64 + ((k >> 3) & 3) * 16 + (n & 15)) * 4 + ((k >> 5) & 3);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = words[4 * j];
+      const float s = (float)((const S*)a.scale)[at + j], z = a.z_on ? (float)a.zero[at + j] : 8.f;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) y[j] += (float)x[p] * (s * ((float)((w >> (4 * (p >> 1) + 16 * (p & 1))) & 15u) - z));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) < INFINITY ? v[j] : y[j];
+  return v;
+}
+
 // bias, residual, activation, rounding of four consecutive outputs
 template <typename T>
 __device__ __forceinline__ void finish4(const Int4Args& a, f32x4 v, int m, int n) {
@@ -267,13 +296,13 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(const Int4Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += t[j];
     }
-    if (a.kz == 1) finish4<T>(a, v, m, n);
+    if (a.kz == 1) finish4<T>(a, plain4<T, S>(a, v, m, n), m, n);
     else *reinterpret_cast<f32x4*>(a.part + ((long long)blockIdx.z * a.M + m) * (tiles * 16) + n) = v;
   }
 }
 
 // Sums the parts of K and finishes: a thread per four outputs.
-template <typename T>
+template <typename T, typename S>
 __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
   const int Np = (a.N + 15) & ~15, per = Np >> 2;
   const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -285,7 +314,7 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += t[j];
   }
-  finish4<T>(a, v, m, n);
+  finish4<T>(a, plain4<T, S>(a, v, m, n), m, n);
 }
 
 template <typename T, typename S, int R, int CT, int G>
@@ -295,7 +324,7 @@ static void launch4(const Int4Args& a, int nw, hipStream_t stream) {
   hipLaunchKernelGGL((int4_linear_kernel<T, S, R, CT, G>), grid, dim3(nw * a.kw * 64), nw * a.kw * R * CT * 1024, stream, a);
   if (a.kz > 1) {
     const long long items = (long long)a.M * ((a.N + 15) / 16 * 4);
-    hipLaunchKernelGGL(int4_join_kernel<T>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((int4_join_kernel<T, S>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
   }
 }
 template <typename T, typename S, int R, int CT>
@@ -335,7 +364,7 @@ extern "C" int dlamd_int4_linear(const void* x, long long x_rs, const void* w, c
   if (kz < 1 || kz > 64 || (kz > 1 && (!part || ((uintptr_t)part & 15) || part_floats < (long long)kz * M * ((N + 15) / 16 * 16)))) return -7;
   if (kz > 1 && (long long)M * ((N + 15) / 16 * 4) > 0xffffff00LL) return -8;      // a launch has fewer than 2^32 threads
   Int4Args a{x, (const uint32_t*)w, scale, (const uint8_t*)zero, (const float*)bias, res, y, x_rs, res_rs, (float*)part,
-             M, N, K, act, kw, kz, zero ? 1 : 0};
+             M, N, K, G, act, kw, kz, zero ? 1 : 0};
   if (dtype == 0 && sdtype == 0) launch4_r<bf16_t, bf16_t>(a, tiles, CT, G, nw, stream);
   if (dtype == 0 && sdtype == 1) launch4_r<bf16_t, f16_t>(a, tiles, CT, G, nw, stream);
   if (dtype == 1 && sdtype == 0) launch4_r<f16_t, bf16_t>(a, tiles, CT, G, nw, stream);

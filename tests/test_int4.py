@@ -281,3 +281,51 @@ def test_shapes_of_the_rule(i):
     res = torch.randn(rows, n, generator=g).to(dt) if has_res else None
     xd, rd = to("cuda", x, res)
     check(Q.linear_int4(xd, w.to("cuda"), res=rd).cpu(), x, codes, scale, z, group, None, "none", res)
+
+
+# ---------------------------------------------------------------------------------------------- odd rows
+def odd_rows(dt, k):
+    """Rows with infinities and NaN, and, in bf16, near the end of the type's range; one ordinary row behind them."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(7, k, generator=g)
+    x[0, 3], x[1, k - 1] = math.inf, -math.inf
+    x[2, 0], x[2, k // 2] = math.inf, math.inf
+    x[3, 40] = math.nan
+    big = 3e38 if dt == torch.bfloat16 else 6e4
+    x[4, 5], x[4, 90], x[5, 50] = big, -big, big
+    return x.to(dt)
+
+
+def check_odd(got, x, codes, scale, z, group, act="none"):
+    """Infinities and NaN where the formula has them (a weight of 0 times infinity among them); elsewhere half a step, 2^-14
+    of the sum of |x w| for sums of up to 1000 products in fp32, and the codes' offset as in ``check``: an output whose weights
+    are all 0 is the difference of two sums of |x| offset, each with 16 roundings of 2^-24."""
+    w = weights64(codes, scale, z, group)
+    y = x.double() @ w.t()
+    ref = act64(y, act)
+    top = torch.finfo(x.dtype).max
+    assert bool((ref.abs() < top)[torch.isfinite(ref)].all())
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isposinf(got), torch.isposinf(ref))
+    assert torch.equal(torch.isneginf(got), torch.isneginf(ref))
+    ok = torch.isfinite(ref)
+    mass = x.double().abs().nan_to_num(0, 0, 0)
+    off = 128 if x.dtype == torch.bfloat16 else 1024
+    tol = torch.finfo(x.dtype).eps / 2 * ref.abs() + 2.0 ** -14 * (mass @ w.abs().t()) + 2.0 ** -24
+    tol += 2.0 ** -24 * 16 * (off + 16) * (mass @ scale.double().repeat_interleave(group, 1).t())
+    assert bool(((got.double() - ref).abs()[ok] <= tol[ok]).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("k,group,shape", [(256, 64, None), (160, 32, None), (640, 128, (1, 1, 4, 3)), (640, 64, (1, 2, 2, 1))])
+def test_infinite_and_largest_rows(k, group, shape, zero, dt, dev, monkeypatch):
+    monkeypatch.setattr(Q, "_SHAPE", shape)
+    codes, scale, z, w = layer(8, 83, k, group, zero, torch.bfloat16)
+    codes[:4] = 8 if z is None else z[:4].repeat_interleave(group, 1)           # outputs whose weights are all 0
+    w = Q.pack_int4(codes[:, 0::2] | (codes[:, 1::2] << 4), scale, z)
+    x = odd_rows(DTYPES[dt], k)
+    check_odd(Q.linear_int4(x.to(dev), w.to(dev)).cpu(), x, codes, scale, z, group)
+    more = torch.cat((x, x, x))                                                  # the kernels for more than 16 rows
+    if shape is None:
+        check_odd(Q.linear_int4(more.to(dev), w.to(dev)).cpu(), more, codes, scale, z, group)
