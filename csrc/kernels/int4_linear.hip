@@ -196,7 +196,7 @@ __device__ __forceinline__ void finish4(const Int4Args& a, f32x4 v, int m, int n
       float f = v[j];
       if (a.bias) f += a.bias[n + j];
       if (a.res) f += (float)rs[j];
-      o[j] = (T)dlamd_act(f, a.act);
+      o[j] = (T)(a.act == ACT_RELU ? (f < 0.f ? 0.f : f) : dlamd_act(f, a.act));      // NaN stays NaN
     }
   }
   if ((a.N & 3) == 0) {

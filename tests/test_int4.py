@@ -329,3 +329,18 @@ def test_infinite_and_largest_rows(k, group, shape, zero, dt, dev, monkeypatch):
     more = torch.cat((x, x, x))                                                  # the kernels for more than 16 rows
     if shape is None:
         check_odd(Q.linear_int4(more.to(dev), w.to(dev)).cpu(), more, codes, scale, z, group)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("act", ["relu", "gelu"])
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_nan_stays_nan_behind_an_activation(dt, act, dev):
+    codes, scale, z, w = layer(8, 40, 128, 64, False, torch.bfloat16)
+    x = torch.randn(4, 128, generator=torch.Generator().manual_seed(2)).to(DTYPES[dt])
+    x[2, 17] = math.nan
+    bias = torch.zeros(40)
+    bias[9] = math.nan
+    got = Q.linear_int4(x.to(dev), w.to(dev), bias.to(dev), act=act).cpu()
+    want = torch.zeros(4, 40, dtype=torch.bool)
+    want[2], want[:, 9] = True, True
+    assert torch.equal(torch.isnan(got), want)
