@@ -4,14 +4,16 @@
 // small next to them.  Weights lie in the order in which a wave takes them for 16x16x32 matrix instructions:
 //     word[N / 16][K / 128][lane][i]   lane = 16 g + r, i < 4:  row 16 t + r, k = 128 s + 32 i + 8 g + (0 .. 7)
 // so a lane's 16-byte load holds its operands of four instructions and a wave's load is 1 KB in one piece.  Inside a word
-// code 2 p lies in bits 4 p and code 2 p + 1 in bits 16 + 4 p: (word >> 4 p) & 0x000f000f is a pair in two 16-bit halves.
+// code 2 p lies in bits 4 p and code 2 p + 1 in bits 16 + 4 p: a shift and a mask give a pair in two 16-bit halves.
 // Scales and zeros are [K / G][N rounded up to 16].
 //
-// A code becomes an operand with one AND-OR: c | 0x4300 is 128 + c in bf16, c | 0x6400 is 1024 + c in fp16, both exact.
-// The offset leaves again after each group of G features,
-//     sum x (c - z) = sum x (off + c) - (off + z) sum x,
+// A code becomes an operand with a shift and one AND-OR: in the top bits of the mantissa of 16 (bits 3 .. 6 in bf16, 6 .. 9 in
+// fp16) it is 16 + c, exactly.  The offset leaves again after each group of G features,
+//     sum x (c - z) = sum x (16 + c) - (16 + z) sum x,
 // where sum x comes from one more matrix instruction (its other operand is all ones), so scale and zero cost one fused
-// multiply-add per group and output, not one per weight.  All sums are fp32.  An infinity in x would make that difference
+// multiply-add per group and output, not one per weight.  All sums are fp32; at this offset the difference is as exact as a
+// sum of the weights' own products (1 to 3e-7 of a layer's typical output).  In the lowest bits codes would need one shift less
+// and stand for 128 + c and 1024 + c: 24 x 8192 x 28672 39.6 instead of 40.2 us, and 1e-6 and 2e-5 off.  An infinity in x would make that difference
 // NaN, and so would bf16 values near the end of their range, whose sums with the offset overflow: an output that is no
 // finite number is summed once more without the offset (plain4).
 //
@@ -42,14 +44,14 @@ struct Int4Args {
 template <typename T> struct Mat4;
 template <> struct Mat4<bf16_t> {
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
-  static constexpr uint32_t BITS = 0x43004300u, ONE = 0x3f803f80u;
-  static constexpr float OFF = 128.f;
+  static constexpr uint32_t BITS = 0x41804180u, ONE = 0x3f803f80u;
+  static constexpr int AT = 3;                               // bit of 1 in a number from 16 to 32
   static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mat4<f16_t> {
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
-  static constexpr uint32_t BITS = 0x64006400u, ONE = 0x3c003c00u;
-  static constexpr float OFF = 1024.f;
+  static constexpr uint32_t BITS = 0x4c004c00u, ONE = 0x3c003c00u;
+  static constexpr int AT = 6;
   static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
@@ -115,12 +117,19 @@ __device__ __forceinline__ void load_rest_tail(Step<R, CT, G>& t, const Int4Args
     }
 }
 
+// Codes 2 p and 2 p + 1 of a word as a pair of numbers 16 + code.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(uint32_t w, uint32_t mask, int p) {
+  constexpr int AT = Mat4<T>::AT;
+  return ((4 * p < AT ? w << (AT - 4 * p) : w >> (4 * p - AT)) & mask) | Mat4<T>::BITS;
+}
+
 template <typename T, typename S, int R, int CT, int G>
 __device__ __forceinline__ void use_step(f32x4 (&y)[R][CT], const u32x4 (&words)[R], const Step<R, CT, G>& t) {
   typedef typename Mat4<T>::x8 x8;
-  constexpr uint32_t BITS = Mat4<T>::BITS, ONE = Mat4<T>::ONE;
-  uint32_t nib = 0x000f000fu;
-  asm("" : "+v"(nib));                                       // in a vector register: AND-OR takes one scalar operand only
+  constexpr uint32_t ONE = Mat4<T>::ONE;
+  uint32_t mask = 0x000f000fu << Mat4<T>::AT;
+  asm("" : "+v"(mask));                                      // in a vector register: AND-OR takes one scalar operand only
   const x8 ones = __builtin_bit_cast(x8, u32x4{ONE, ONE, ONE, ONE});
 #pragma unroll
   for (int q = 0; q < 128 / G; ++q) {
@@ -138,7 +147,7 @@ __device__ __forceinline__ void use_step(f32x4 (&y)[R][CT], const u32x4 (&words)
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         const uint32_t w = words[i][i4];
-        const u32x4 v = {(w & nib) | BITS, ((w >> 4) & nib) | BITS, ((w >> 8) & nib) | BITS, ((w >> 12) & nib) | BITS};
+        const u32x4 v = {pair_of<T>(w, mask, 0), pair_of<T>(w, mask, 1), pair_of<T>(w, mask, 2), pair_of<T>(w, mask, 3)};
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[i][c] = Mat4<T>::mul(__builtin_bit_cast(x8, v), __builtin_bit_cast(x8, t.x[c][i4]), acc[i][c]);
       }
@@ -149,7 +158,7 @@ __device__ __forceinline__ void use_step(f32x4 (&y)[R][CT], const u32x4 (&words)
       for (int j = 0; j < 4; ++j) {
         const uint32_t h = j & 1 ? t.s[i][q][j >> 1] >> 16 : t.s[i][q][j >> 1] & 0xffffu;
         const float s = (float)__builtin_bit_cast(S, (uint16_t)h);
-        const float z = Mat4<T>::OFF + (float)((t.z[i][q] >> (8 * j)) & 0xffu);
+        const float z = 16.f + (float)((t.z[i][q] >> (8 * j)) & 0xffu);
 #pragma unroll
         for (int c = 0; c < CT; ++c) y[i][c][j] += s * (acc[i][c][j] - z * xs[c][j]);
       }

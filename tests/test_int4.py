@@ -299,7 +299,7 @@ def odd_rows(dt, k):
 def check_odd(got, x, codes, scale, z, group, act="none"):
     """Infinities and NaN where the formula has them (a weight of 0 times infinity among them); elsewhere half a step, 2^-14
     of the sum of |x w| for sums of up to 1000 products in fp32, and the codes' offset as in ``check``: an output whose weights
-    are all 0 is the difference of two sums of |x| offset, each with 16 roundings of 2^-24."""
+    are all 0 is the difference of two sums of 16 to 31 |x|, each with 16 roundings of 2^-24."""
     w = weights64(codes, scale, z, group)
     y = x.double() @ w.t()
     ref = act64(y, act)
@@ -309,9 +309,8 @@ def check_odd(got, x, codes, scale, z, group, act="none"):
     assert torch.equal(torch.isneginf(got), torch.isneginf(ref))
     ok = torch.isfinite(ref)
     mass = x.double().abs().nan_to_num(0, 0, 0)
-    off = 128 if x.dtype == torch.bfloat16 else 1024
     tol = torch.finfo(x.dtype).eps / 2 * ref.abs() + 2.0 ** -14 * (mass @ w.abs().t()) + 2.0 ** -24
-    tol += 2.0 ** -24 * 16 * (off + 16) * (mass @ scale.double().repeat_interleave(group, 1).t())
+    tol += 2.0 ** -24 * 16 * 32 * (mass @ scale.double().repeat_interleave(group, 1).t())
     assert bool(((got.double() - ref).abs()[ok] <= tol[ok]).all())
 
 
@@ -344,3 +343,28 @@ def test_nan_stays_nan_behind_an_activation(dt, act, dev):
     want = torch.zeros(4, 40, dtype=torch.bool)
     want[2], want[:, 9] = True, True
     assert torch.equal(torch.isnan(got), want)
+
+
+# ---------------------------------------------------------------------------------------------- bits of the sums
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("k,group", [(1024, 64), (8192, 128), (4096, 32)])
+def test_sums_keep_32_bits(k, group, dt, dev):
+    """Rows of positive numbers (behind relu), whose sum is far larger than the output: what a code is shifted by on its way into
+    the products must not eat the sum's bits.  The bias is the negated result, so the output is the error, in fine steps.
+    A group of q = G / 32 matrix instructions has at most 8 q full-size roundings in each of its two sums of up to 31 sum |x|,
+    spread evenly over half a step of 2^-24: sqrt(16 q / 12) 31 2^-24 s sum |x| per group, added up over groups as independent
+    errors are, and the output's own sum (a rounding of 2^-24 of it per group, and the bias)."""
+    codes, scale, z, w = layer(3, 600, k, group, False, torch.bfloat16)
+    g = torch.Generator().manual_seed(4)
+    x = (torch.rand(6, k, generator=g) + 0.5).to(DTYPES[dt])
+    big = scale * 64                                             # errors well above the output type's last step
+    w = Q.pack_int4(codes[:, 0::2] | (codes[:, 1::2] << 4), big).to(dev)
+    ref = x.double() @ weights64(codes, big, None, group).t()
+    mass = x.double().view(6, 1, k // group, group).sum(-1) * big.double()             # [6, 600, groups]
+    bound = math.sqrt(16 * (group // 32) / 12) * 31 * 2.0 ** -24 * mass.pow(2).sum(-1).sqrt()
+    bound = bound + 2.0 ** -24 * math.sqrt(k // group + 2) * ref.abs().amax()
+    err = torch.stack([Q.linear_int4(x[i : i + 1].to(dev), w, -ref[i].float().to(dev)).cpu().double()[0] - (ref[i] - ref[i].float().double())
+                       for i in range(6)])
+    rms, most = float((err / bound).pow(2).mean().sqrt()), float((err / bound).abs().max())
+    assert rms <= 1.0 and most <= 6.0, (rms, most)                # 3600 outputs: six standard deviations
