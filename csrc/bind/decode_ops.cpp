@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -80,10 +81,14 @@ void same_device(const c10::Device& d, std::initializer_list<const at::Tensor*> 
   for (const at::Tensor* t : ts) need(!t || t->device() == d, "all tensors live on one device");
 }
 
-// The operators have no backward: a result that silently carried no gradient would train nothing.
+// The operators have no derivatives: a result that silently carried no gradient would train nothing, one without its tangent
+// would be a constant in forward mode (which torch.no_grad() leaves on).
 void no_gradient(std::initializer_list<const at::Tensor*> ts) {
-  if (c10::GradMode::is_enabled())
-    for (const at::Tensor* t : ts) need(!t || !t->requires_grad(), "the operator has no gradient: call it under torch.no_grad() or on detached tensors");
+  const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const at::Tensor* t : ts) {
+    need(!backward || !t || !t->requires_grad(), "the operator has no gradient: call it under torch.no_grad() or on detached tensors");
+    need(!forward || !t || !t->_fw_grad(0).defined(), "the operator has no forward-mode derivative: call it on detached tensors");
+  }
 }
 
 int half_type(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : -1; }

@@ -18,6 +18,7 @@ from pathlib import Path
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB: Optional[ctypes.CDLL] = None
 _LOCK = threading.Lock()
@@ -85,9 +86,12 @@ def bind():
 
 
 def no_gradient(*ts: Optional[torch.Tensor]) -> None:
-    """For operators without a backward: a result that silently carried no gradient would train nothing."""
+    """For operators without derivatives: a result that silently carried no gradient would train nothing, one without its
+    tangent would be a constant in forward mode (which torch.no_grad() leaves on)."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise ValueError("the operator has no gradient: call it under torch.no_grad() or on detached tensors")
+    if torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError("the operator has no forward-mode derivative: call it on detached tensors")
 
 
 def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:

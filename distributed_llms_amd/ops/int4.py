@@ -122,7 +122,7 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
                 res: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = act(x @ W^T + bias (+ res)) in x's type.  x: [..., K] bf16 or fp16, bias: fp32 [N], res: [..., N] of x's type;
     act: none, relu, gelu.  Products are exact and summed in fp32, rounded once.  No gradient: x, bias and res that require
-one are refused outside torch.no_grad()."""
+    one are refused outside torch.no_grad(), and so are those with a forward-mode tangent."""
     code = _ACTS.get(act)
     if code is None:
         raise ValueError("act is none, relu or gelu")

@@ -18,7 +18,7 @@ accepted plus one - the rejected tokens' slots are simply written again).
 
 Everything runs on the current stream of the tensors' device, allocates only through PyTorch and reads no device value on
 the host, so a decode step can be captured in a hipGraph and replayed while ``lens`` advances.  Neither operator has a
-gradient; tensors that require one are refused outside torch.no_grad().
+gradient; tensors that require one are refused outside torch.no_grad(), and so are tensors with a forward-mode tangent.
 """
 from __future__ import annotations
 

@@ -368,3 +368,22 @@ def test_sums_keep_32_bits(k, group, dt, dev):
                        for i in range(6)])
     rms, most = float((err / bound).pow(2).mean().sqrt()), float((err / bound).abs().max())
     assert rms <= 1.0 and most <= 6.0, (rms, most)                # 3600 outputs: six standard deviations
+
+
+@pytest.mark.parametrize("dev", ["checks", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("why", ["x", "bias", "res"])
+def test_refuses_tangents(why, dev):
+    """Dual tensors of forward-mode differentiation: the result would come back without its tangent."""
+    from distributed_llms_amd.ops import _loader
+
+    if dev == "checks" and not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    at = "cuda" if dev == "cuda" else "cpu"
+    c = dict(x=torch.zeros(2, 64, dtype=torch.bfloat16, device=at), bias=torch.zeros(40, device=at), res=torch.zeros(2, 40, dtype=torch.bfloat16, device=at))
+    w = layer(0, 40, 64, 32, False, torch.bfloat16)[3].to(at)
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        c[why] = torch.autograd.forward_ad.make_dual(c[why], torch.ones_like(c[why]))
+        with pytest.raises(ValueError):
+            Q.linear_int4(c["x"], w, c["bias"], res=c["res"])
+        with pytest.raises(ValueError):
+            _loader.bind().linear_int4(c["x"], w.words, w.scale, w.zero, w.n, w.k, w.group, c["bias"], 0, c["res"], None, 0)

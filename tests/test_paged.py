@@ -740,3 +740,32 @@ def test_a_key_with_an_infinite_component_weighs_nothing(n, D, dt):
         out.append(P.paged_attention(**{x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}, return_lse=True))
     assert torch.isfinite(out[0][0]).all() and torch.equal(out[0][1], out[1][1])
     assert torch.equal(out[0][0].view(torch.int16), out[1][0].view(torch.int16))
+
+
+# ---------------------------------------------------------------------------------------------- forward mode
+@pytest.mark.parametrize("dev", BINDING)
+@pytest.mark.parametrize("why", ["q", "k_pages", "v_pages"])
+def test_attention_refuses_tangents(why, dev):
+    """Dual tensors of forward-mode differentiation: the result would come back without its tangent.  torch.no_grad() leaves
+    forward mode on."""
+    c = {"scale": None, "causal": True, **att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True)}
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        c[why] = torch.autograd.forward_ad.make_dual(c[why].cuda() if dev == "cuda" else c[why], torch.ones_like(c[why], device=dev if dev == "cuda" else "cpu"))
+        refused_by_the_binding(dev, c, lambda bind, d: bind.paged_attention(
+            *(d[x] for x in ("q", "k_pages", "v_pages", "table", "lens", "scale", "causal")), None, False, None, 0, 0))
+        if dev == "checks":
+            with pytest.raises(ValueError):
+                P.paged_attention(**c)
+
+
+@pytest.mark.parametrize("dev", BINDING)
+@pytest.mark.parametrize("why", ["k", "v", "q", "k_pages"])
+def test_append_refuses_tangents(why, dev):
+    c = {"q": None, "cos": None, "sin": None, "starts": None, "interleaved": False, **_append_args()}
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        c[why] = torch.autograd.forward_ad.make_dual(c[why].cuda() if dev == "cuda" else c[why], torch.ones_like(c[why], device=dev if dev == "cuda" else "cpu"))
+        refused_by_the_binding(dev, c, lambda bind, d: bind.paged_append(
+            *(d[x] for x in ("k", "v", "k_pages", "v_pages", "table", "lens", "q", "cos", "sin", "starts", "interleaved")), 0))
+        if dev == "checks":
+            with pytest.raises(ValueError):
+                P.paged_append(**c)
