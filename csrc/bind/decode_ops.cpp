@@ -119,7 +119,7 @@ PyObject* append(PyObject* const* a) {
   need(k.scalar_type() == dt && v.scalar_type() == dt && k.stride(2) == 1 && v.stride(2) == 1,
        "k and v have the cache's type and a contiguous last dimension");
   need(D % 8 == 0 && hkv > 0, "D is a multiple of 8, the cache has heads");
-  no_gradient({&k, &v, &kp, &vp, q.t});
+  no_gradient({&k, &v, &kp, &vp, q.t, cos.t, sin.t});
   same_device(k.device(), {&v, &kp, &vp, &table, &lens, q.t, cos.t, sin.t, starts.t});
   if (q)
     need(q->dim() == 3 && q->size(0) == T && q->size(1) > 0 && q->size(2) == D && q->scalar_type() == dt && q->stride(2) == 1,
@@ -323,7 +323,7 @@ PyObject* int4(PyObject* const* a) {
            half_type(scale.scalar_type()) >= 0 && scale.is_contiguous() && scale.numel() == K / G * ((N + 15) / 16 * 16) &&
            (!zero || (zero->scalar_type() == at::kByte && zero->is_contiguous() && zero->numel() == scale.numel())),
        "words, scale and zero are not those of an [N, K] layer as pack_int4 lays it out");
-  no_gradient({&x, bias.t, res.t});
+  no_gradient({&x, &scale, bias.t, res.t});
   same_device(x.device(), {&words, &scale, zero.t, bias.t, res.t});
   const Where w(x, a[11]);
   at::Tensor x2 = dims == 2 ? x : x.reshape({-1, K}), r2;

@@ -121,7 +121,7 @@ def _bind():
 def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None, *, act: str = "none",
                 res: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = act(x @ W^T + bias (+ res)) in x's type.  x: [..., K] bf16 or fp16, bias: fp32 [N], res: [..., N] of x's type;
-    act: none, relu, gelu.  Products are exact and summed in fp32, rounded once.  No gradient: x, bias and res that require
+    act: none, relu, gelu.  Products are exact and summed in fp32, rounded once.  No gradient: x, scales, bias and res that require
     one are refused outside torch.no_grad(), and so are those with a forward-mode tangent."""
     code = _ACTS.get(act)
     if code is None:
@@ -135,7 +135,7 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
         raise ValueError("bias is fp32 [N]")
     if res is not None and (res.shape[:-1] != x.shape[:-1] or res.shape[-1] != w.n or res.dtype != x.dtype):
         raise ValueError("res is [..., N] of x's type")
-    _loader.no_gradient(x, bias, res)
+    _loader.no_gradient(x, w.scale, bias, res)
     if any(t is not None and t.device != x.device for t in (w.words, bias, res)):
         raise ValueError("all tensors live on one device")
     return linear_int4_reference(x, w, bias, act, res).to(x.dtype)

@@ -125,7 +125,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         raise ValueError("k and v have the cache's type and a contiguous last dimension")
     if D % 8 != 0 or hkv == 0:
         raise ValueError("D is a multiple of 8, the cache has heads")
-    _loader.no_gradient(k, v, k_pages, v_pages, q)
+    _loader.no_gradient(k, v, k_pages, v_pages, q, cos, sin)
     if any(x is not None and x.device != k.device for x in (v, k_pages, v_pages, table, lens, q, cos, sin, starts)):
         raise ValueError("all tensors live on one device")
     if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[1] == 0 or q.shape[2] != D or q.dtype != dt or q.stride(2) != 1):

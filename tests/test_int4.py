@@ -387,3 +387,20 @@ def test_refuses_tangents(why, dev):
             Q.linear_int4(c["x"], w, c["bias"], res=c["res"])
         with pytest.raises(ValueError):
             _loader.bind().linear_int4(c["x"], w.words, w.scale, w.zero, w.n, w.k, w.group, c["bias"], 0, c["res"], None, 0)
+
+
+@pytest.mark.parametrize("dev", ["checks", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_refuses_scales_that_require_a_gradient(dev):
+    from distributed_llms_amd.ops import _loader
+
+    if dev == "checks" and not _loader.kernels_available():
+        pytest.skip("the kernel library is not built")
+    at = "cuda" if dev == "cuda" else "cpu"
+    x, scale = torch.zeros(2, 64, dtype=torch.bfloat16, device=at), torch.ones(40, 2, dtype=torch.bfloat16, device=at, requires_grad=True)
+    w = Q.pack_int4(torch.zeros(40, 32, dtype=torch.uint8, device=at), scale)
+    with pytest.raises(ValueError):
+        Q.linear_int4(x, w)
+    with pytest.raises(ValueError):
+        _loader.bind().linear_int4(x, w.words, w.scale, w.zero, w.n, w.k, w.group, None, 0, None, None, 0)
+    with torch.no_grad():
+        assert Q.linear_int4(x, w).shape == (2, 40)

@@ -769,3 +769,13 @@ def test_append_refuses_tangents(why, dev):
         if dev == "checks":
             with pytest.raises(ValueError):
                 P.paged_append(**c)
+
+
+@pytest.mark.parametrize("dev", BINDING)
+def test_append_refuses_rotation_tables_that_require_a_gradient(dev):
+    c = {"q": None, "cos": None, "sin": None, "starts": None, "interleaved": False, **_append_args()}
+    c["sin"] = c["sin"].clone().requires_grad_()
+    with pytest.raises(ValueError):
+        P.paged_append(**c)
+    refused_by_the_binding(dev, c, lambda bind, d: bind.paged_append(
+        *(d[x] for x in ("k", "v", "k_pages", "v_pages", "table", "lens", "q", "cos", "sin", "starts", "interleaved")), 0))
