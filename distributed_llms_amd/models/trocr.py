@@ -225,9 +225,7 @@ class TrOCR(nn.Module):
         served better by bf16.  The encoder and the cross-attention keys / values (hundreds of rows per crop) stay bf16."""
         self.eval()
         cfg = self.cfg
-        if int4_group is not None:
-            self.int4_group = int4_group
-        g4 = self.int4_group
+        g4 = self.int4_group if int4_group is None else int4_group
         dec = (lambda lin: _pk4(lin, g4)) if g4 else _pk
         dev = self.lm_head.weight.device
         pk: Dict = {}
@@ -252,7 +250,7 @@ class TrOCR(nn.Module):
         lb = torch.full((cfg.vocab_padded,), -1e4, device=dev)
         lb[: cfg.vocab] = 0.0
         pk["lm"] = (quantize_int4(lw, g4) if g4 else lw.to(torch.bfloat16).contiguous(), lb.contiguous())
-        self._pk = pk
+        self._pk, self.int4_group = pk, g4                                 # together: a refused group changes nothing
         self._graphs = {}
         return self
 

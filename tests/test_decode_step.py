@@ -279,3 +279,22 @@ def test_rules_give_what_the_entries_take():
         b, v = log(1 << 22), log(1 << 29)
         pieces = rules.rule_pieces(b, v)
         assert 1 <= pieces <= 64 and (pieces == 1 or b <= 65535)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_refused_group_changes_nothing(dev):
+    """Sizes of groups that no layer has: the weights packed before, or none, and the earlier choice stand."""
+    _, xin = image(SMALL, 2, dev)
+    m = model(SMALL).to(dev)
+    for bad in (48, 256):
+        with pytest.raises(ValueError):
+            m.prepare(int4_group=bad)
+    toks, _ = m.generate(xin, max_len=4)
+    assert m.int4_group == 0 and not isinstance(m._pk["lm"][0], Q.Int4Weight)
+    m.prepare(int4_group=32)
+    four, _ = m.generate(xin, max_len=4)
+    with pytest.raises(ValueError):
+        m.prepare(int4_group=48)
+    assert m.int4_group == 32 and torch.equal(m.generate(xin, max_len=4)[0], four)
+    m = m.to(dev)                               # packed weights are dropped; the choice stays
+    assert torch.equal(m.generate(xin, max_len=4)[0], four) and m._pk["lm"][0].group == 32
