@@ -162,7 +162,7 @@ class TrOCR(nn.Module):
             elif isinstance(m, nn.Embedding):
                 nn.init.normal_(m.weight, std=0.02)
         self._pk: Optional[Dict] = None
-        self._graphs: Dict[int, "_DecodeGraph"] = {}
+        self._graphs: Dict[Tuple[int, bool], "_DecodeGraph"] = {}          # (batch bucket, captured)
         self.int4_group = 0
 
     def _apply(self, fn, *a, **k):
@@ -329,10 +329,10 @@ class TrOCR(nn.Module):
         B = x.shape[0]
         on_gpu = x.is_cuda
         Bb = B if not on_gpu else max(16, 1 << (B - 1).bit_length())
-        g = self._graphs.get(Bb)
+        capture = on_gpu and use_graph
+        g = self._graphs.get((Bb, capture))
         if g is None:
-            g = _DecodeGraph(self, Bb, capture=on_gpu and use_graph)
-            self._graphs[Bb] = g
+            g = self._graphs[Bb, capture] = _DecodeGraph(self, Bb, capture)
         st = g.state
         # encoder and the cross-attention K/V of every layer, once per batch, a chunk of crops at a time
         for c0 in range(0, B, self.ENC_CHUNK):

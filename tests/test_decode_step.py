@@ -298,3 +298,18 @@ def test_a_refused_group_changes_nothing(dev):
     assert m.int4_group == 32 and torch.equal(m.generate(xin, max_len=4)[0], four)
     m = m.to(dev)                               # packed weights are dropped; the choice stays
     assert torch.equal(m.generate(xin, max_len=4)[0], four) and m._pk["lm"][0].group == 32
+
+
+@pytest.mark.gpu
+def test_without_a_graph_nothing_is_replayed():
+    """Eager steps after captured ones, and the other way round: each call does as it is told, with the same tokens."""
+    _, xin = image(SMALL, 3, "cuda")
+    for first in (True, False):
+        m, want = model(SMALL).cuda().prepare(), None
+        replays = lambda: sum(g.replays for g in m._graphs.values())  # noqa: E731
+        for use_graph in (first, not first, first):
+            before = replays()
+            toks, conf = m.generate(xin, use_graph=use_graph, eos_check_every=0)
+            assert replays() - before == (SMALL.max_len if use_graph else 0)
+            want = want or (toks, conf)
+            assert torch.equal(toks, want[0]) and torch.equal(conf, want[1])
