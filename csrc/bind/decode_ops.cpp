@@ -91,6 +91,10 @@ void no_gradient(std::initializer_list<const at::Tensor*> ts) {
   }
 }
 
+// A dimension of one element has whatever stride: none is asked of it, and none is passed on.
+bool packed(const at::Tensor& t, int d) { return t.size(d) < 2 || t.stride(d) == 1; }
+ll step(const at::Tensor& t, int d) { return t.size(d) < 2 ? 0 : t.stride(d); }
+
 int half_type(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : -1; }
 
 void check_cache(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& table, const at::Tensor& lens) {
@@ -98,7 +102,7 @@ void check_cache(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& t
   need(half_type(kp.scalar_type()) >= 0 && vp.scalar_type() == kp.scalar_type(), "the cache is bf16 or fp16");
   need(table.dim() == 2 && table.scalar_type() == at::kInt && lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == table.size(0),
        "table is int32 [B, width], lens int32 [B]");
-  need(kp.stride(3) == 1 && vp.stride(3) == 1 && table.stride(1) == 1 && lens.stride(0) == 1,
+  need(packed(kp, 3) && packed(vp, 3) && packed(table, 1) && packed(lens, 0),
        "the last dimensions of the cache, of table and of lens have to be contiguous");
 }
 int as_int(int64_t v) {
@@ -116,13 +120,13 @@ PyObject* append(PyObject* const* a) {
   need(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == hkv && k.size(2) == D, "k and v are [T, kv_heads, D] with the cache's heads and D");
   const int64_t T = k.size(0);
   const at::ScalarType dt = kp.scalar_type();
-  need(k.scalar_type() == dt && v.scalar_type() == dt && k.stride(2) == 1 && v.stride(2) == 1,
+  need(k.scalar_type() == dt && v.scalar_type() == dt && packed(k, 2) && packed(v, 2),
        "k and v have the cache's type and a contiguous last dimension");
   need(D % 8 == 0 && hkv > 0, "D is a multiple of 8, the cache has heads");
   no_gradient({&k, &v, &kp, &vp, q.t, cos.t, sin.t});
   same_device(k.device(), {&v, &kp, &vp, &table, &lens, q.t, cos.t, sin.t, starts.t});
   if (q)
-    need(q->dim() == 3 && q->size(0) == T && q->size(1) > 0 && q->size(2) == D && q->scalar_type() == dt && q->stride(2) == 1,
+    need(q->dim() == 3 && q->size(0) == T && q->size(1) > 0 && q->size(2) == D && q->scalar_type() == dt && packed(*q.t, 2),
          "q is [T, heads, D] of the cache's type and device with a contiguous last dimension");
   need((bool)cos == (bool)sin, "cos and sin come together");
   int64_t rot = 0;
@@ -134,16 +138,16 @@ PyObject* append(PyObject* const* a) {
          "cos and sin are contiguous fp32");
   }
   if (starts)
-    need(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == B + 1 && starts->stride(0) == 1,
+    need(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == B + 1 && packed(*starts.t, 0),
          "starts is int32 [B + 1] on the cache's device");
   else
     need((B ? T % B : T) == 0, "without starts every sequence has the same number of new tokens");
   const Where w(k, a[11]);
   at::Tensor qo;
   if (q) qo = B && width ? at::empty({T, q->size(1), D}, q->options()) : at::zeros({T, q->size(1), D}, q->options());
-  launched(k_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), q.ptr(), q ? q->stride(0) : 0,
-                    q ? q->stride(1) : 0, q ? qo.data_ptr() : nullptr, kp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2), vp.data_ptr(),
-                    vp.stride(0), vp.stride(1), vp.stride(2), table.data_ptr(), table.stride(0), lens.data_ptr(), starts.ptr(), cos.ptr(),
+  launched(k_append(k.data_ptr(), step(k, 0), step(k, 1), v.data_ptr(), step(v, 0), step(v, 1), q.ptr(), q ? step(*q.t, 0) : 0,
+                    q ? step(*q.t, 1) : 0, q ? qo.data_ptr() : nullptr, kp.data_ptr(), step(kp, 0), step(kp, 1), step(kp, 2), vp.data_ptr(),
+                    step(vp, 0), step(vp, 1), step(vp, 2), table.data_ptr(), step(table, 0), lens.data_ptr(), starts.ptr(), cos.ptr(),
                     sin.ptr(), as_int(B), as_int(T), q ? as_int(q->size(1)) : 0, as_int(hkv), as_int(D), (int)rot, as_int(page), as_int(width),
                     as_int(kp.size(0)), truth(a[10]), half_type(dt), w.stream),
            "dlamd_paged_append");
@@ -190,7 +194,7 @@ int64_t row_groups(int64_t rows, int64_t heads, int64_t bound) {
 PyObject* attention(PyObject* const* a) {
   const at::Tensor &q = tensor(a[0]), &kp = tensor(a[1]), &vp = tensor(a[2]), &table = tensor(a[3]), &lens = tensor(a[4]);
   check_cache(kp, vp, table, lens);
-  need(q.dim() == 4 && q.scalar_type() == kp.scalar_type() && q.stride(3) == 1,
+  need(q.dim() == 4 && q.scalar_type() == kp.scalar_type() && packed(q, 3),
        "q is [B, n, heads, D] of the cache's type with a contiguous last dimension");
   const int64_t B = q.size(0), n = q.size(1), hq = q.size(2), D = q.size(3), page = kp.size(1), hkv = kp.size(2), width = table.size(1);
   need(table.size(0) == B && kp.size(3) == D && hkv > 0 && hq % hkv == 0,
@@ -218,8 +222,8 @@ PyObject* attention(PyObject* const* a) {
   const bool want = truth(a[8]);
   if (want) lse = at::empty({B, n, hq}, q.options().dtype(at::kFloat));
   if (d.share) part = at::empty({d.share + problems, rows, D + 4}, q.options().dtype(at::kFloat));
-  launched(k_attention(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), kp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
-                       vp.data_ptr(), vp.stride(0), vp.stride(1), vp.stride(2), table.data_ptr(), table.stride(0), lens.data_ptr(),
+  launched(k_attention(q.data_ptr(), step(q, 0), step(q, 1), step(q, 2), kp.data_ptr(), step(kp, 0), step(kp, 1), step(kp, 2),
+                       vp.data_ptr(), step(vp, 0), step(vp, 1), step(vp, 2), table.data_ptr(), step(table, 0), lens.data_ptr(),
                        o.data_ptr(), want ? lse.data_ptr() : nullptr, d.share ? part.data_ptr() : nullptr, d.share ? part.numel() : 0, as_int(groups), as_int(d.share), as_int(d.least),
                        as_int(B), as_int(n), as_int(hq), as_int(hkv), as_int(D), as_int(page), as_int(width), as_int(kp.size(0)), truth(a[6]),
                        (float)scale, half_type(q.scalar_type()), w.stream),
@@ -254,11 +258,11 @@ PyObject* verify(PyObject* const* a) {
   const int64_t V = target.size(2);
   if (proposal)
     need(proposal->dim() == 3 && proposal->size(0) == B && proposal->size(1) == n && proposal->size(2) == V && proposal->scalar_type() == dt &&
-             proposal->stride(2) == 1,
+             packed(*proposal.t, 2),
          "proposal is [B, n, V] of the target's type, rows contiguous");
-  need(u.dim() == 2 && u.size(0) == B && u.size(1) == n + 1 && u.scalar_type() == at::kFloat && u.stride(1) == 1, "u is fp32 [B, n + 1]");
-  if (counts) need(counts->dim() == 1 && counts->size(0) == B && counts->scalar_type() == at::kInt && counts->stride(0) == 1, "counts is int32 [B]");
-  need(target.stride(2) == 1 && draft.stride(1) == 1, "the last dimension of target and draft has to be contiguous");
+  need(u.dim() == 2 && u.size(0) == B && u.size(1) == n + 1 && u.scalar_type() == at::kFloat && packed(u, 1), "u is fp32 [B, n + 1]");
+  if (counts) need(counts->dim() == 1 && counts->size(0) == B && counts->scalar_type() == at::kInt && packed(*counts.t, 0), "counts is int32 [B]");
+  need(packed(target, 2) && packed(draft, 1), "the last dimension of target and draft has to be contiguous");
   same_device(draft.device(), {&target, &u, proposal.t, counts.t});
   const ll pad = number(a[5]);
   need(pad >= -0x80000000LL && pad <= 0x7fffffffLL, "pad is an int32");
@@ -267,8 +271,8 @@ PyObject* verify(PyObject* const* a) {
   const bool with_q = proposal && n > 0;
   const int64_t pieces = a[6] == Py_None ? pieces_of(B, V, V * target.element_size() * (with_q ? 2 : 1)) : number(a[6]);
   if (pieces > 1) sums = at::empty({B, pieces, 2}, draft.options().dtype(at::kDouble));
-  launched(k_verify(draft.data_ptr(), draft.stride(0), target.data_ptr(), target.stride(0), target.stride(1), with_q ? proposal.ptr() : nullptr,
-                    with_q ? proposal->stride(0) : 0, with_q ? proposal->stride(1) : 0, u.data_ptr(), u.stride(0), counts.ptr(),
+  launched(k_verify(draft.data_ptr(), step(draft, 0), target.data_ptr(), step(target, 0), step(target, 1), with_q ? proposal.ptr() : nullptr,
+                    with_q ? step(*proposal.t, 0) : 0, with_q ? step(*proposal.t, 1) : 0, u.data_ptr(), step(u, 0), counts.ptr(),
                     tokens.data_ptr(), accepted.data_ptr(), pieces > 1 ? sums.data_ptr() : nullptr, pieces > 1 ? sums.numel() : 0, as_int(pieces), as_int(B), as_int(n),
                     as_int(V), (int)pad, type, w.stream),
            "dlamd_verify_draft");
@@ -314,7 +318,7 @@ PyObject* int4(PyObject* const* a) {
   const int type = half_type(x.scalar_type());
   const int64_t dims = x.dim();
   need(dims > 0 && x.size(dims - 1) == K && type >= 0, "x is [..., K] bf16 or fp16");
-  if (bias) need(bias->dim() == 1 && bias->size(0) == N && bias->scalar_type() == at::kFloat && bias->stride(0) == 1, "bias is fp32 [N]");
+  if (bias) need(bias->dim() == 1 && bias->size(0) == N && bias->scalar_type() == at::kFloat && packed(*bias.t, 0), "bias is fp32 [N]");
   if (res)
     need(res->dim() == dims && res->size(dims - 1) == N && res->sizes().slice(0, dims - 1) == x.sizes().slice(0, dims - 1) &&
              res->scalar_type() == x.scalar_type(),
@@ -327,11 +331,11 @@ PyObject* int4(PyObject* const* a) {
   same_device(x.device(), {&words, &scale, zero.t, bias.t, res.t});
   const Where w(x, a[11]);
   at::Tensor x2 = dims == 2 ? x : x.reshape({-1, K}), r2;
-  if (x2.stride(1) != 1 || x2.stride(0) % 8 != 0 || x2.stride(0) >= 1 << 24 || ((uintptr_t)x2.data_ptr() & 15))
+  if (x2.stride(1) != 1 || step(x2, 0) % 8 != 0 || step(x2, 0) >= 1 << 24 || ((uintptr_t)x2.data_ptr() & 15))
     x2 = x2.clone(at::MemoryFormat::Contiguous);             // rows the kernel cannot load 16 bytes at a time or address
   if (res) {
     r2 = dims == 2 ? *res.t : res->reshape({-1, N});
-    if (r2.stride(1) != 1) r2 = r2.contiguous();
+    if (!packed(r2, 1)) r2 = r2.contiguous();
   }
   const int64_t M = x2.size(0);
   c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
@@ -344,8 +348,8 @@ PyObject* int4(PyObject* const* a) {
          (int)number(PyTuple_GET_ITEM(a[10], 3))};
   }
   if (s.kz > 1) part = at::empty({s.kz, M, (N + 15) / 16 * 16}, x.options().dtype(at::kFloat));
-  launched(k_int4(x2.data_ptr(), x2.stride(0), words.data_ptr(), scale.data_ptr(), zero.ptr(), bias.ptr(), res ? r2.data_ptr() : nullptr,
-                  res ? r2.stride(0) : 0, y.data_ptr(), as_int(M), as_int(N), as_int(K), as_int(G), (int)number(a[8]), type,
+  launched(k_int4(x2.data_ptr(), step(x2, 0), words.data_ptr(), scale.data_ptr(), zero.ptr(), bias.ptr(), res ? r2.data_ptr() : nullptr,
+                  res ? step(r2, 0) : 0, y.data_ptr(), as_int(M), as_int(N), as_int(K), as_int(G), (int)number(a[8]), type,
                   half_type(scale.scalar_type()), s.tiles, s.nw, s.kw, s.kz, s.kz > 1 ? part.data_ptr() : nullptr, s.kz > 1 ? part.numel() : 0, w.stream),
            "dlamd_int4_linear");
   return THPVariable_Wrap(std::move(y));

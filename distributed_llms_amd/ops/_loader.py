@@ -85,6 +85,11 @@ def bind():
     return _BIND
 
 
+def packed(t: torch.Tensor, dim: int) -> bool:
+    """Neighbours along ``dim`` are neighbours in memory (a dimension of one element has whatever stride)."""
+    return t.shape[dim] < 2 or t.stride(dim) == 1
+
+
 def no_gradient(*ts: Optional[torch.Tensor]) -> None:
     """For operators without derivatives: a result that silently carried no gradient would train nothing, one without its
     tangent would be a constant in forward mode (which torch.no_grad() leaves on)."""

@@ -93,13 +93,13 @@ def verify_draft(draft: torch.Tensor, target: torch.Tensor, u: torch.Tensor, pro
         raise ValueError(f"at most {MAX_DRAFTED} drafted tokens")
     if target.dim() != 3 or target.shape[:2] != (B, n + 1) or dt not in (torch.bfloat16, torch.float16, torch.float32) or target.shape[2] == 0:
         raise ValueError("target is [B, n + 1, V] bf16, fp16 or fp32")
-    if proposal is not None and (proposal.shape != (B, n, target.shape[2]) or proposal.dtype != dt or proposal.stride(2) != 1):
+    if proposal is not None and (proposal.shape != (B, n, target.shape[2]) or proposal.dtype != dt or not _loader.packed(proposal, 2)):
         raise ValueError("proposal is [B, n, V] of the target's type, rows contiguous")
-    if u.shape != (B, n + 1) or u.dtype != torch.float32 or u.stride(1) != 1:
+    if u.shape != (B, n + 1) or u.dtype != torch.float32 or not _loader.packed(u, 1):
         raise ValueError("u is fp32 [B, n + 1]")
-    if counts is not None and (counts.shape != (B,) or counts.dtype != torch.int32 or counts.stride(0) != 1):
+    if counts is not None and (counts.shape != (B,) or counts.dtype != torch.int32 or not _loader.packed(counts, 0)):
         raise ValueError("counts is int32 [B]")
-    if target.stride(2) != 1 or draft.stride(1) != 1:
+    if not (_loader.packed(target, 2) and _loader.packed(draft, 1)):
         raise ValueError("the last dimension of target and draft has to be contiguous")
     if any(x is not None and x.device != draft.device for x in (target, u, proposal, counts)):
         raise ValueError("all tensors live on one device")

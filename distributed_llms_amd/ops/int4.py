@@ -131,7 +131,7 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
                                               _loader.raw_stream(x.get_device()))
     if x.dim() == 0 or x.shape[-1] != w.k or x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("x is [..., K] bf16 or fp16")
-    if bias is not None and (bias.shape != (w.n,) or bias.dtype != torch.float32 or bias.stride(0) != 1):
+    if bias is not None and (bias.shape != (w.n,) or bias.dtype != torch.float32 or not _loader.packed(bias, 0)):
         raise ValueError("bias is fp32 [N]")
     if res is not None and (res.shape[:-1] != x.shape[:-1] or res.shape[-1] != w.n or res.dtype != x.dtype):
         raise ValueError("res is [..., N] of x's type")

@@ -94,7 +94,7 @@ def _check_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
         raise ValueError("the cache is bf16 or fp16")
     if table.dtype != torch.int32 or lens.dtype != torch.int32 or table.dim() != 2 or lens.shape != table.shape[:1]:
         raise ValueError("table is int32 [B, width], lens int32 [B]")
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1 or table.stride(1) != 1 or lens.stride(0) != 1:
+    if not all(_loader.packed(t, -1) for t in (k_pages, v_pages, table, lens)):
         raise ValueError("the last dimensions of the cache, of table and of lens have to be contiguous")
 
 
@@ -121,14 +121,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if k.dim() != 3 or k.shape != v.shape or k.shape[1] != hkv or k.shape[2] != D:
         raise ValueError("k and v are [T, kv_heads, D] with the cache's heads and D")
     T = k.shape[0]
-    if k.dtype != dt or v.dtype != dt or k.stride(2) != 1 or v.stride(2) != 1:
+    if k.dtype != dt or v.dtype != dt or not (_loader.packed(k, 2) and _loader.packed(v, 2)):
         raise ValueError("k and v have the cache's type and a contiguous last dimension")
     if D % 8 != 0 or hkv == 0:
         raise ValueError("D is a multiple of 8, the cache has heads")
     _loader.no_gradient(k, v, k_pages, v_pages, q, cos, sin)
     if any(x is not None and x.device != k.device for x in (v, k_pages, v_pages, table, lens, q, cos, sin, starts)):
         raise ValueError("all tensors live on one device")
-    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[1] == 0 or q.shape[2] != D or q.dtype != dt or q.stride(2) != 1):
+    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[1] == 0 or q.shape[2] != D or q.dtype != dt or not _loader.packed(q, 2)):
         raise ValueError("q is [T, heads, D] of the cache's type and device with a contiguous last dimension")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
@@ -137,7 +137,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < width * page or rot > D or rot % 16 != 0:
             raise ValueError("cos and sin are [P, rot / 2] with P >= width * page, rot <= D and rot % 16 == 0")
     if starts is not None:
-        if starts.dtype != torch.int32 or starts.shape != (B + 1,) or starts.stride(0) != 1:
+        if starts.dtype != torch.int32 or starts.shape != (B + 1,) or not _loader.packed(starts, 0):
             raise ValueError("starts is int32 [B + 1] on the cache's device")
     elif (T % B if B else T) != 0:
         raise ValueError("without starts every sequence has the same number of new tokens")
@@ -194,7 +194,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         return (_BIND or _bind()).paged_attention(q, k_pages, v_pages, table, lens, scale, causal, max_len, return_lse, *_DEAL,
                                                   _loader.raw_stream(q.get_device()))
     _check_cache(k_pages, v_pages, table, lens)
-    if q.dim() != 4 or q.dtype != k_pages.dtype or q.stride(3) != 1:
+    if q.dim() != 4 or q.dtype != k_pages.dtype or not _loader.packed(q, 3):
         raise ValueError("q is [B, n, heads, D] of the cache's type with a contiguous last dimension")
     B, n, hq, D = q.shape
     page, hkv, kD = k_pages.shape[1:]

@@ -216,3 +216,16 @@ def test_the_last_token_stands_for_the_end_of_the_row(V, pieces, monkeypatch):
     p[torch.arange(V)[None, None] > last[:, None, None]] = 0.0
     tokens, accepted = verify_draft(torch.zeros(60, 0, dtype=torch.int32, device="cuda"), p.cuda(), torch.ones(60, 1, device="cuda"))
     assert torch.equal(tokens.cpu()[:, 0].long(), last) and not bool(accepted.any())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_one_draft_of_any_stride(dev):
+    """A dimension of one element may have any stride: one draft, one number, one count taken out of larger tensors."""
+    strided = lambda x, *st: torch.empty_strided(x.shape, st, dtype=x.dtype, device=dev).copy_(x)  # noqa: E731
+    c = case(3, 6, 1, 700, torch.float32)
+    same(verify_draft(**{**on(c, dev), "draft": strided(c["draft"], 1, 6)}), plain(**c))
+    c = case(4, 1, 0, 700, torch.float32)
+    same(verify_draft(**{**on(c, dev), "u": strided(c["u"], 9, 5), "counts": strided(c["counts"], 3)}), plain(**c))
+    c = case(5, 4, 2, 1, torch.float32)
+    d = {**on(c, dev), "target": strided(c["target"], 12, 3, 2), "proposal": strided(c["proposal"], 12, 3, 2)}
+    same(verify_draft(**d), plain(**c))

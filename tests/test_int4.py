@@ -404,3 +404,15 @@ def test_refuses_scales_that_require_a_gradient(dev):
         _loader.bind().linear_int4(x, w.words, w.scale, w.zero, w.n, w.k, w.group, None, 0, None, None, 0)
     with torch.no_grad():
         assert Q.linear_int4(x, w).shape == (2, 40)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_one_output_and_one_row_of_any_stride(dev):
+    codes, scale, z, w = layer(5, 1, 64, 32, False, torch.bfloat16)
+    x = torch.randn(1, 64, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    bias, res = torch.randn(3, generator=torch.Generator().manual_seed(3))[::3], torch.ones(1, 7, dtype=torch.bfloat16)[:, ::7]
+    assert bias.stride() == (3,) and res.stride(1) == 7
+    xd = torch.empty_strided((1, 64), (13, 1), dtype=torch.bfloat16, device=dev).copy_(x)
+    bd = torch.empty_strided((1,), (3,), device=dev).copy_(bias)
+    rd = torch.empty_strided((1, 1), (7, 7), dtype=torch.bfloat16, device=dev).copy_(res)
+    check(Q.linear_int4(xd, w.to(dev), bd, res=rd).cpu(), x, codes, scale, z, 32, bias, "none", res)

@@ -779,3 +779,25 @@ def test_append_refuses_rotation_tables_that_require_a_gradient(dev):
         P.paged_append(**c)
     refused_by_the_binding(dev, c, lambda bind, d: bind.paged_append(
         *(d[x] for x in ("k", "v", "k_pages", "v_pages", "table", "lens", "q", "cos", "sin", "starts", "interleaved")), 0))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_one_sequence_of_any_stride(dev):
+    """A dimension of one element may have any stride: one sequence, one page, one token, one head."""
+    c = att_case(4, [5], 1, 16, 1, 1, 64, torch.bfloat16, True)
+    c["k_pages"], c["v_pages"], c["table"] = c["k_pages"][:1], c["v_pages"][:1], torch.zeros(1, 1, dtype=torch.int32)
+    c["k_pages"], c["v_pages"] = c["k_pages"].nan_to_num(1.0), c["v_pages"].nan_to_num(1.0, 1.0, 1.0)
+    new = torch.randn(2, 1, 1, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    want = {x: y.clone() if torch.is_tensor(y) else y for x, y in c.items()}
+    P.paged_append(new[0], new[1], want["k_pages"], want["v_pages"], want["table"], want["lens"])
+    ref, _ = P.paged_attention_reference(**want, dtype=torch.float64)
+
+    def odd(x):                                                     # every dimension of one element with a stride of its own
+        y = torch.empty_strided(x.shape, [s if n > 1 else 13 + 2 * i for i, (n, s) in enumerate(zip(x.shape, x.stride()))], dtype=x.dtype, device=dev)
+        return y.copy_(x)
+
+    d = {x: odd(y) if torch.is_tensor(y) else y for x, y in c.items()}
+    P.paged_append(odd(new[0]), odd(new[1]), d["k_pages"], d["v_pages"], d["table"], d["lens"])
+    assert torch.equal(d["k_pages"].cpu(), want["k_pages"]) and torch.equal(d["v_pages"].cpu(), want["v_pages"])
+    o = P.paged_attention(**d)
+    assert bool(((o.cpu().double() - ref).abs() <= att_tolerance(c, ref)).all())
