@@ -11,6 +11,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../kernels/decode_abi.h"
@@ -84,7 +85,8 @@ void same_device(const c10::Device& d, std::initializer_list<const at::Tensor*> 
 // The operators have no derivatives: a result that silently carried no gradient would train nothing, one without its tangent
 // would be a constant in forward mode (which torch.no_grad() leaves on).
 void no_gradient(std::initializer_list<const at::Tensor*> ts) {
-  const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  const bool backward = c10::GradMode::is_enabled();
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0);
   for (const at::Tensor* t : ts) {
     need(!backward || !t || !t->requires_grad(), "the operator has no gradient: call it under torch.no_grad() or on detached tensors");
     need(!forward || !t || !t->_fw_grad(0).defined(), "the operator has no forward-mode derivative: call it on detached tensors");
