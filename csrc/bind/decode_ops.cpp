@@ -70,7 +70,14 @@ ll number(PyObject* o) {
   }
   return v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    throw Refused("a truth value is expected");
+  }
+  return v == 1;
+}
 
 // Device of the call, made current for the launch, and its current stream as Python knows it.
 struct Where {

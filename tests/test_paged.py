@@ -801,3 +801,19 @@ def test_one_sequence_of_any_stride(dev):
     assert torch.equal(d["k_pages"].cpu(), want["k_pages"]) and torch.equal(d["v_pages"].cpu(), want["v_pages"])
     o = P.paged_attention(**d)
     assert bool(((o.cpu().double() - ref).abs() <= att_tolerance(c, ref)).all())
+
+
+class Undecided:
+    def __bool__(self):
+        raise TypeError("neither true nor false")
+
+
+def test_the_device_path_wants_truth_values():
+    """A flag that cannot say whether it is true is refused before anything is launched."""
+    c = {"scale": None, **att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True)}
+    for causal, want in ((Undecided(), False), (True, Undecided())):
+        refused_by_the_binding("checks", c, lambda bind, d: bind.paged_attention(
+            *(d[x] for x in ("q", "k_pages", "v_pages", "table", "lens", "scale")), causal, None, want, None, 0, 0))
+    a = {"q": None, "cos": None, "sin": None, "starts": None, **_append_args()}
+    refused_by_the_binding("checks", a, lambda bind, d: bind.paged_append(
+        *(d[x] for x in ("k", "v", "k_pages", "v_pages", "table", "lens", "q", "cos", "sin", "starts")), Undecided(), 0))
