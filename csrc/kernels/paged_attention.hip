@@ -60,10 +60,10 @@ struct PagedAttArgs {
 #define LN2 0.6931471805599453f
 
 // mul: a 16x16x32 product; split: two weights as 16-bit halves hi + lo (hi may be rounded either way, lo makes up for it); UP:
-// weights are 2^UP exp(score - maximum).
+// weights are 2^UP exp(score - maximum), DOWN is 2^-UP.
 template <typename T> struct Mat;
 template <> struct Mat<bf16_t> {
-  static constexpr float UP = 0.f;
+  static constexpr float UP = 0.f, DOWN = 1.f;
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
   typedef __bf16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -75,7 +75,7 @@ template <> struct Mat<bf16_t> {
   static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mat<f16_t> {
-  static constexpr float UP = 14.f;
+  static constexpr float UP = 14.f, DOWN = 1.f / 16384.f;
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
         T* dst = (T*)p.o + to * D + d0;
 #pragma unroll
         for (int d = 0; d < D / 16; d += 4) *reinterpret_cast<u32x2*>(dst + d) = *reinterpret_cast<u32x2*>(t + d);
-        if (p.lse && d0 == 0) p.lse[to] = sum == 0.f ? -INFINITY : (m * p.scale2 + (__log2f(sum) - Mat<T>::UP)) * LN2;
+        if (p.lse && d0 == 0) p.lse[to] = sum == 0.f ? -INFINITY : (m * p.scale2 + __log2f(sum * Mat<T>::DOWN)) * LN2;
       } else {
         float* dst = part + in * (D + 4);
 #pragma unroll
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
       v += f * s_o[x][threadIdx.x];
     }
     ((T*)p.o)[to * D + threadIdx.x] = (T)(sum2 == 0.f ? 0.f : v / sum2);
-    if (p.lse && threadIdx.x == 0) p.lse[to] = sum2 == 0.f ? -INFINITY : (top * p.scale2 + (__log2f(sum2) - Mat<T>::UP)) * LN2;
+    if (p.lse && threadIdx.x == 0) p.lse[to] = sum2 == 0.f ? -INFINITY : (top * p.scale2 + __log2f(sum2 * Mat<T>::DOWN)) * LN2;
   }
 }
 

@@ -817,3 +817,58 @@ def test_the_device_path_wants_truth_values():
     a = {"q": None, "cos": None, "sin": None, "starts": None, **_append_args()}
     refused_by_the_binding("checks", a, lambda bind, d: bind.paged_append(
         *(d[x] for x in ("k", "v", "k_pages", "v_pages", "table", "lens", "q", "cos", "sin", "starts")), Undecided(), 0))
+
+
+# ---------------------------------------------------------------------------------------------- every key once
+def counting_case(kept, n, page, hq, hkv, D, dt, causal, seed):
+    """All scores 0, so a row's weights are 1 / keys seen; dimension d has the value 1024 at one position and 0 elsewhere.  The
+    positions lie beside the borders of half tiles, tiles, waves, pages and likely parts, and at both ends."""
+    g = torch.Generator().manual_seed(seed)
+    need = [max(k, 0) + (n if causal and k >= 0 else 0) for k in kept]
+    table, pages = tables(need, page, g)
+    kp = torch.randn(pages, page, hkv, D, generator=g).to(dt)
+    vp = torch.zeros(pages, page, hkv, D, dtype=dt)
+    want = torch.zeros(len(kept), n, hkv, D, dtype=torch.float64)
+    for b, m in enumerate(need):
+        if m == 0:
+            continue
+        near = sorted({p for s in (16, 32, 128, page, 1024, m) for x in range(0, m + 1, s) for p in (x - 1, x) if 0 <= p < m})
+        ends = near[:4] + near[-n - 4 :]
+        pick = torch.randint(0, len(near), (hkv, D), generator=g)
+        for h in range(hkv):
+            for d in range(D):
+                pos = ends[d] if d < len(ends) else near[int(pick[h, d])]
+                vp[int(table[b, pos // page]), pos % page, h, d] = 1024.0
+                for i in range(n):
+                    seen = max(kept[b], 0) + (i + 1 if causal else 0)
+                    if pos < seen:
+                        want[b, i, h, d] = 1024.0 / seen
+    c = dict(q=torch.zeros(len(kept), n, hq, D, dtype=dt), k_pages=kp, v_pages=vp, table=table, lens=torch.tensor(kept, dtype=torch.int32), causal=causal)
+    return c, want.repeat_interleave(hq // hkv, 2)
+
+
+COUNT = [  # kept, n, page, hq, hkv, D, dtype, causal
+    ([3001, 0, 127, 128, 2047], 1, 48, 4, 2, 64, "bf16", True),
+    ([1500, 777, -1, 16, 5000], 5, 16, 16, 2, 128, "fp16", True),
+    ([2900, 33, 4096], 1, 256, 3, 3, 128, "bf16", False),
+    ([640, 6001], 40, 64, 2, 2, 64, "fp16", True),
+    ([100] * 3 + [9000] + [1] * 30, 3, 32, 12, 2, 64, "bf16", True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(COUNT)))
+@pytest.mark.parametrize("share,least", [(None, 0), (0, 0), (1, 1), (7, 3), (64, 1), (700, 1), (256, 1)])
+def test_attention_kernel_takes_every_key_once(case, share, least, monkeypatch):
+    """A key that is lost shows as 0, one that is taken twice as twice the value.  Weights are equal powers of two and sums of
+    them exact; the division and the output each round once.  The log-sum-exp is a logarithm to base 2 below 16 (last place
+    2^-20, times ln 2), times an ln 2 that is off by 2^-25 (2^-21 in all), rounded (2^-21): 2^-19 together."""
+    kept, n, page, hq, hkv, D, dt, causal = COUNT[case]
+    c, want = counting_case(kept, n, page, hq, hkv, D, DTYPES[dt], causal, case)
+    monkeypatch.setattr(P, "_DEAL", (share, least))
+    o, lse = P.paged_attention(**{x: y.cuda() if torch.is_tensor(y) else y for x, y in c.items()}, return_lse=True)
+    err = (o.cpu().double() - want).abs()
+    assert bool((err <= (torch.finfo(DTYPES[dt]).eps / 2 + 2.0 ** -21) * want).all()), (err.max(), torch.nonzero(err > 0.01 * want)[:5])
+    seen = (torch.tensor(kept).clamp(min=0)[:, None] + (torch.arange(1, n + 1) if causal else torch.zeros(n))) * (torch.tensor(kept) >= 0)[:, None]
+    assert bool(((lse.cpu().double() - seen.double().log()[..., None]).nan_to_num(0.0).abs() <= 2.0 ** -19).all())
+    assert torch.equal(torch.isneginf(lse.cpu()), (seen == 0)[..., None].expand(lse.shape))
