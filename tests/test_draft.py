@@ -229,3 +229,16 @@ def test_one_draft_of_any_stride(dev):
     c = case(5, 4, 2, 1, torch.float32)
     d = {**on(c, dev), "target": strided(c["target"], 12, 3, 2), "proposal": strided(c["proposal"], 12, 3, 2)}
     same(verify_draft(**d), plain(**c))
+
+
+def test_distribution_is_the_targets_on_the_cpu():
+    """As above, through the operator itself: five standard deviations of 3000 draws."""
+    N, V = 3000, 6
+    g = torch.Generator().manual_seed(8)
+    p, q = (torch.randn(V, generator=g).softmax(-1) for _ in range(2))
+    draft = torch.multinomial(q, N, replacement=True, generator=g).to(torch.int32)[:, None]
+    tokens, accepted = verify_draft(draft, p.expand(N, 2, V), torch.rand(N, 2, generator=g), proposal=q.expand(N, 1, V))
+    freq = torch.bincount(tokens[:, 0].long(), minlength=V).double() / N
+    assert bool(((freq - p).abs() <= 5 * (p * (1 - p) / N).sqrt()).all())
+    rate = torch.minimum(p, q).sum()                                          # of accepted drafts
+    assert abs(float(accepted.double().mean() - rate)) <= 5 * float((rate * (1 - rate) / N).sqrt())
