@@ -313,3 +313,25 @@ def test_without_a_graph_nothing_is_replayed():
             assert replays() - before == (SMALL.max_len if use_graph else 0)
             want = want or (toks, conf)
             assert torch.equal(toks, want[0]) and torch.equal(conf, want[1])
+
+
+@pytest.mark.gpu
+def test_recognizer_over_its_whole_length():
+    """Sequences that cannot end: every token up to the last position, across page borders and beyond 1024, is compared with the
+    PyTorch model; the captured step and the eager one give the same."""
+    cfg = dataclasses.replace(SMALL, max_len=1100)
+    models = [model(cfg, seed=1) for _ in range(2)]
+    for m in models:
+        with torch.no_grad():
+            m.lm_head.weight[cfg.eos] = 0.0                    # a logit of 0 never is the largest of 300
+    x, xin = image(cfg, 2, "cuda")
+    m = models[1].cuda().prepare()
+    toks, conf = m.generate(xin)
+    assert toks.shape == (2, 1100) and not bool((toks == cfg.eos).any()) and m.last_decode_steps == 1100
+    near = check_tokens(models[0], x, toks)
+    for part in (slice(0, 64), slice(64, 1024), slice(1024, 1100)):
+        assert near[:, part].float().mean().item() > 0.9, part
+    before = sum(g.replays for g in m._graphs.values())
+    eager, econf = m.generate(xin, use_graph=False)
+    assert sum(g.replays for g in m._graphs.values()) == before
+    assert torch.equal(eager, toks) and torch.equal(econf, conf)
