@@ -218,7 +218,7 @@ PyObject* attention(PyObject* const* a) {
       PyErr_Clear();
       throw Refused("scale is a number");
     }
-    need(std::isfinite((float)scale), "scale is a finite number");
+    need(std::fabs(scale) <= 2e38, "scale is a number of at most 2e38");        // its product with log2(e) fits 32 bits
   }
   int64_t bound = width * page;
   if (a[7] != Py_None) bound = std::min<int64_t>(bound, number(a[7]));

@@ -51,7 +51,7 @@ struct PagedAttArgs {
   int groups, rows, share, least;                            // row groups per (b, kv head), rows per group; workgroups to deal
                                                              // tiles out to (0: one for each problem), least tiles of a part
   uint32_t page_magic;                                       // ceil(2^32 / (page / 16))
-  float scale2;                                              // |scale| log2(e), above 0
+  float scale2;                                              // |scale| log2(e), above 0: -inf stays -inf
   uint32_t flip;                                             // sign bits to turn in q where the scale is negative
 };
 
@@ -683,7 +683,7 @@ extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_
   const uint32_t magic = units == 1 ? 0u : (uint32_t)((0x100000000ULL + units - 1) / units);
   PagedAttArgs a{q, kp, vp, o, (float*)lse, (float*)part, (const int*)table, (const int*)lens, q_bs, q_ns, q_hs,
                  kp_ps * 2, vp_ps * 2, t_bs, (int)sl[0], (int)sl[2], (int)sl[1], (int)sl[3], B, n, Hq, Hkv, page, width, pages, causal,
-                 groups, rows, share, least, magic, fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f), scale < 0.f ? 0x80008000u : 0u};
+                 groups, rows, share, least, magic, fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f), scale < 0.f ? 0x80008000u : 0u};
   if (dtype == 0 && D == 64) launch_rows<bf16_t, 64>(a, rows, stream);
   if (dtype == 0 && D == 128) launch_rows<bf16_t, 128>(a, rows, stream);
   if (dtype == 1 && D == 64) launch_rows<f16_t, 64>(a, rows, stream);

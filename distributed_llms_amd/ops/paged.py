@@ -189,7 +189,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (cross-attention over encoder tokens held in pages).  A query that sees nothing, or only scores of -inf, gives 0 and a
     log-sum-exp of -inf.
     ``max_len``: an upper bound of the positions any query sees, when the caller knows a tighter one than ``width * page``
-    (only used to choose how the work is split; lengths are read on the device).  D is 64 or 128, page % 16 == 0."""
+    (only used to choose how the work is split; lengths are read on the device).  D is 64 or 128, page % 16 == 0, ``scale``
+    (None: D^-1/2) a number of either sign up to 2e38."""
     if q.is_cuda:
         return (_BIND or _bind()).paged_attention(q, k_pages, v_pages, table, lens, scale, causal, max_len, return_lse, *_DEAL,
                                                   _loader.raw_stream(q.get_device()))
@@ -202,8 +203,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("q, table and cache disagree: one table row per sequence, D alike, heads a multiple of kv_heads")
     if page % 16 != 0 or page == 0 or D not in (64, 128):
         raise ValueError("page is a multiple of 16, D is 64 or 128")
-    if scale is not None and not abs(scale) <= torch.finfo(torch.float32).max:
-        raise ValueError("scale is a finite number")
+    if scale is not None and not abs(scale) <= 2e38:
+        raise ValueError("scale is a number of at most 2e38")
     _loader.no_gradient(q, k_pages, v_pages)
     if any(x.device != q.device for x in (k_pages, v_pages, table, lens)):
         raise ValueError("all tensors live on one device")

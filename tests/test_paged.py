@@ -872,3 +872,26 @@ def test_attention_kernel_takes_every_key_once(case, share, least, monkeypatch):
     seen = (torch.tensor(kept).clamp(min=0)[:, None] + (torch.arange(1, n + 1) if causal else torch.zeros(n))) * (torch.tensor(kept) >= 0)[:, None]
     assert bool(((lse.cpu().double() - seen.double().log()[..., None]).nan_to_num(0.0).abs() <= 2.0 ** -19).all())
     assert torch.equal(torch.isneginf(lse.cpu()), (seen == 0)[..., None].expand(lse.shape))
+
+
+@pytest.mark.parametrize("scale", [2.1e38, -3e38])
+def test_attention_refuses_scales_beyond_its_range(scale):
+    c = {**att_case(1, [3, 4], 1, 16, 4, 2, 64, torch.bfloat16, True), "scale": scale}
+    with pytest.raises(ValueError):
+        P.paged_attention(**c)
+    refused_by_the_binding("checks", c, lambda bind, d: bind.paged_attention(
+        *(d[x] for x in ("q", "k_pages", "v_pages", "table", "lens", "scale", "causal")), None, False, None, 0, 0))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("scale,size", [(1e-36, 1e18), (3e-32, 1e16), (1.9e38, 9e-20), (-1e-36, 1e18), (0.0, 1e14)])
+def test_attention_with_scales_at_the_ends_of_their_range(scale, size, dev):
+    """q and k are as large or small as it takes for scores of some units."""
+    c = att_case(8, [90, 300], 2, 16, 4, 2, 64, torch.bfloat16, True, qscale=0.3)
+    c["q"], c["k_pages"] = (c["q"].float() * size).to(torch.bfloat16), (c["k_pages"].float() * size).to(torch.bfloat16)
+    d = {x: y.to(dev) if torch.is_tensor(y) else y for x, y in c.items()}
+    o, lse = P.paged_attention(**d, scale=scale, return_lse=True)
+    ref, ref_lse = P.paged_attention_reference(**c, scale=scale, dtype=torch.float64)
+    assert bool((ref_lse.abs() < 64).all())
+    assert bool(((o.cpu().double() - ref).abs() <= att_tolerance(c, ref)).all())
+    assert bool(((lse.cpu().double() - ref_lse).abs() <= 2.0 ** -24 * 130 * 64).all())
