@@ -45,8 +45,8 @@ struct PagedAttArgs {
                                                              // word: tiles of a part
   const int *table, *lens;
   long long q_bs, q_ns, q_hs;
-  long long k_ps, v_ps, t_bs;                                // page strides of the cache in bytes; table rows in entries
-  int k_ss, k_hs, v_ss, v_hs;                                // slot / head strides in bytes
+  long long k_ps, k_hs, v_ps, v_hs, t_bs;                    // page / head strides of the cache in bytes; table rows in entries
+  int k_ss, v_ss;                                            // slot strides in bytes
   int B, n, Hq, Hkv, page, width, pages, causal;
   int groups, rows, share, least;                            // row groups per (b, kv head), rows per group; workgroups to deal
                                                              // tiles out to (0: one for each problem), least tiles of a part
@@ -285,8 +285,8 @@ __device__ __forceinline__ void add_values_again(Rows<T, D, MT>& w, const PagedA
       const int pi = key / p.page, pid = row[pi];
       if (pid < 0 || pid >= p.pages) continue;
       const long long slot = key - pi * p.page;
-      const T* kr = (const T*)((const char*)p.kp + pid * p.k_ps + slot * p.k_ss + (long long)hk * p.k_hs);
-      const T* vr = (const T*)((const char*)p.vp + pid * p.v_ps + slot * p.v_ss + (long long)hk * p.v_hs) + D / 4 * g;
+      const T* kr = (const T*)((const char*)p.kp + pid * p.k_ps + slot * p.k_ss + hk * p.k_hs);
+      const T* vr = (const T*)((const char*)p.vp + pid * p.v_ps + slot * p.v_ss + hk * p.v_hs) + D / 4 * g;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const int at = row0 + 16 * mt + r, i = at / G, h = hk * G + at - i * G;
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 3 : MT == 2 ? 2 : 1) void paged_atte
   }
   // The next tile's keys are fetched into the registers of this one's as soon as the scores have been taken, its values
   // after the products: at any time a wave has most of a tile in flight, and three waves fit a SIMD.
-  const global_p kh = (global_p)p.kp + (long long)hk * p.k_hs, vh = (global_p)p.vp + (long long)hk * p.v_hs;
+  const global_p kh = (global_p)p.kp + hk * p.k_hs, vh = (global_p)p.vp + hk * p.v_hs;
   bool odd = false;
   if (k0 < limit) {
     u32x4 k[2][D / 32];
@@ -656,10 +656,9 @@ extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_
   if (page <= 0 || page % 16 != 0 || width < 0 || pages < 0) return -2;
   if ((q_bs | q_ns | q_hs | kp_ps | kp_ss | kp_hs | vp_ps | vp_ss | vp_hs) % 8 != 0) return -3;
   if (((uintptr_t)q | (uintptr_t)kp | (uintptr_t)vp | (uintptr_t)o) & 15) return -4;
-  // a lane's offset inside 16 slots is a 24-bit product, a head's and a page's inside one page 32 bits
-  const long long sl[4] = {kp_ss * 2, vp_ss * 2, kp_hs * 2, vp_hs * 2};
-  if (sl[0] < 0 || sl[1] < 0 || sl[0] >= (1 << 24) || sl[1] >= (1 << 24) || sl[2] < 0 || sl[3] < 0 || sl[2] > 0x7fffffff ||
-      sl[3] > 0x7fffffff || page * sl[0] > 0x7fffffff || page * sl[1] > 0x7fffffff)
+  // a lane's offset inside 16 slots is a 24-bit product, a slot's inside its page 32 bits
+  const long long sl[2] = {kp_ss * 2, vp_ss * 2};
+  if (sl[0] < 0 || sl[1] < 0 || sl[0] >= (1 << 24) || sl[1] >= (1 << 24) || page * sl[0] > 0x7fffffff || page * sl[1] > 0x7fffffff)
     return -11;
   // positions are 32-bit; the page of a position is a multiplication, exact while units * (page / 16) < 2^32
   if ((long long)width * page > 0x7ff00000LL || (long long)width * (page / 16) * (page / 16) >= (1LL << 32)) return -5;
@@ -682,7 +681,7 @@ extern "C" int dlamd_paged_attention(const void* q, long long q_bs, long long q_
   const uint32_t units = (uint32_t)(page / 16);
   const uint32_t magic = units == 1 ? 0u : (uint32_t)((0x100000000ULL + units - 1) / units);
   PagedAttArgs a{q, kp, vp, o, (float*)lse, (float*)part, (const int*)table, (const int*)lens, q_bs, q_ns, q_hs,
-                 kp_ps * 2, vp_ps * 2, t_bs, (int)sl[0], (int)sl[2], (int)sl[1], (int)sl[3], B, n, Hq, Hkv, page, width, pages, causal,
+                 kp_ps * 2, kp_hs * 2, vp_ps * 2, vp_hs * 2, t_bs, (int)sl[0], (int)sl[1], B, n, Hq, Hkv, page, width, pages, causal,
                  groups, rows, share, least, magic, fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f), scale < 0.f ? 0x80008000u : 0u};
   if (dtype == 0 && D == 64) launch_rows<bf16_t, 64>(a, rows, stream);
   if (dtype == 0 && D == 128) launch_rows<bf16_t, 128>(a, rows, stream);

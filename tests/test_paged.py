@@ -895,3 +895,29 @@ def test_attention_with_scales_at_the_ends_of_their_range(scale, size, dev):
     assert bool((ref_lse.abs() < 64).all())
     assert bool(((o.cpu().double() - ref).abs() <= att_tolerance(c, ref)).all())
     assert bool(((lse.cpu().double() - ref_lse).abs() <= 2.0 ** -24 * 130 * 64).all())
+
+
+@pytest.mark.gpu
+def test_attention_kernel_heads_more_than_2_gb_apart():
+    """Heads outside pages and slots, as views of a buffer that holds more than 2^31 bytes of each head."""
+    g = torch.Generator().manual_seed(12)
+    far, pages, page, hkv, D = (1 << 30) + 8 * 64, 5, 16, 2, 64
+    views = []
+    for _ in range(2):
+        buf = torch.zeros(far + pages * page * D, dtype=torch.bfloat16, device="cuda")
+        views.append(buf.as_strided((pages, page, hkv, D), (page * D, D, far, 1)))
+    small = [torch.randn(pages, page, hkv, D, generator=g).to(torch.bfloat16) for _ in range(2)]
+    for x, y in zip(views, small):
+        x.copy_(y)
+    table, lens = torch.tensor([[4, 0, 2], [3, 1, -1]], dtype=torch.int32), torch.tensor([40, 20], dtype=torch.int32)
+    q = torch.randn(2, 1, 4, D, generator=g).to(torch.bfloat16)
+    new = [torch.randn(2, hkv, D, generator=g).to(torch.bfloat16) for _ in range(2)]
+    P.paged_append(*(x.cuda() for x in new), *views, table.cuda(), lens.cuda())
+    P.paged_append(*new, *small, table, lens)
+    assert torch.equal(views[0].cpu(), small[0]) and torch.equal(views[1].cpu(), small[1])
+    o = P.paged_attention(q.cuda(), *views, table.cuda(), lens.cuda()).cpu()
+    c = dict(q=q, k_pages=small[0], v_pages=small[1], table=table, lens=lens, causal=True)
+    ref, _ = P.paged_attention_reference(**c, dtype=torch.float64)
+    assert bool(((o.double() - ref).abs() <= att_tolerance(c, ref)).all())
+    del views, buf
+    torch.cuda.empty_cache()
