@@ -187,6 +187,7 @@ __device__ __forceinline__ f32x4 plain4(const Int4Args& a, f32x4 v, int m, int n
 #pragma unroll
       for (int p = 0; p < 8; ++p) y[j] += (float)x[p] * (s * ((float)((w >> (4 * (p >> 1) + 16 * (p & 1))) & 15u) - z));
     }
+    if (y[0] != y[0] && y[1] != y[1] && y[2] != y[2] && y[3] != y[3]) break;       // NaN in x: there is no more to find
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) < INFINITY ? v[j] : y[j];
