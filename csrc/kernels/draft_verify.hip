@@ -10,7 +10,8 @@
 //
 // Two rows per sequence are read once, the drafted probabilities before them (a gather each), the piece with the border after
 // the sums: a chain of dependent fetches, hence rows in registers up to 8192 tokens (8 x 4000: 5.8 us), pieces over several
-// workgroups and a second launch beyond (1 x 50265: 8.0 us, 3.4 + 4.3 on the device; 192 x 50265: 22 us, 3.5 TB/s).
+// workgroups and a second launch beyond (1 x 50265: 9.6 us, 8.0 in a graph, 3.4 + 4.3 on the device; 192 x 50265: 22 us,
+// 3.5 TB/s).
 #include "common.h"
 #include "decode_abi.h"
 

@@ -13,16 +13,20 @@
 // where sum x comes from one more matrix instruction (its other operand is all ones), so scale and zero cost one fused
 // multiply-add per group and output, not one per weight.  All sums are fp32; at this offset the difference is as exact as a
 // sum of the weights' own products (1 to 3e-7 of a layer's typical output).  In the lowest bits codes would need one shift less
-// and stand for 128 + c and 1024 + c: 24 x 8192 x 28672 39.6 instead of 40.2 us, and 1e-6 and 2e-5 off.  An infinity in x would make that difference
+// and stand for 128 + c and 1024 + c: 24 x 8192 x 28672 39.4 instead of 39.9 us, and 1e-6 and 2e-5 off.  An infinity in x would make that difference
 // NaN, and so would bf16 values near the end of their range, whose sums with the offset overflow: an output that is no
-// finite number is summed once more without the offset (plain4).
+// finite number is summed once more without the offset (plain4; 24 x 8192 x 28672 with an infinity in a row: 2.4 ms).
 //
 // The waves of a workgroup share R tiles of 16 outputs and split K between them, 128 features at a time; their sums meet in
 // LDS.  The next step's loads are in flight while a step is computed.
 //
-// 5 x 50265 x 1024: 9.5 us, 2.9 TB/s; 1 x 16384 x 4096: 10.2 us; 24 x 8192 x 28672: 39 us, 3.2 TB/s.  There a stream of the
+// 5 x 50265 x 1024: 9.6 us, 2.9 TB/s; 1 x 16384 x 4096: 10.9 us; 24 x 8192 x 28672: 39.9 us, 3.1 TB/s.  There a stream of the
 // words alone takes 26 us; fetching x (from L2), the scales and the unpacking, scaling and products cost 4 to 8 us each on top,
 // which neither x through LDS for eight waves (40 - 46 us), nor more waves over K (44) or over outputs (41 - 42) hid.
+// Farther from a stream of their words: 17 to 64 rows of middle-sized layers (48 x 11008 x 4096 24 us, 24 x 7000 x 2048 in groups
+// of 64 11.9), where every wave fetches as many bytes of x as of words or more, and from 33 rows on two workgroups fetch and
+// unpack the same words; groups of 32 (1 x 20000 x 8192 36.6 us, in groups of 128 22.6), with as many loads of scales and
+// zeros as of words; hundreds of rows (600 x 4096 x 4096 59 us), where a word is unpacked again for each 32.
 #include "common.h"
 #include "decode_abi.h"
 
@@ -339,7 +343,8 @@ static void launch4(const Int4Args& a, int nw, hipStream_t stream) {
 }
 template <typename T, typename S, int R, int CT>
 static void launch4_g(const Int4Args& a, int G, int nw, hipStream_t stream) {
-  constexpr int R32 = R * CT == 8 ? 2 : R;                   // the scales of groups of 32 and 8 tiles do not fit the registers
+  constexpr int R32 = R * CT == 8 ? 2 : R;                   // the scales of groups of 32 and 8 tiles do not fit the registers;
+                                                             // of groups of 64 all but 10 to 17 do, which go to scratch
   if (G == 32) launch4<T, S, R32, CT, 32>(a, nw, stream);
   else if (G == 64) launch4<T, S, R, CT, 64>(a, nw, stream);
   else launch4<T, S, R, CT, 128>(a, nw, stream);

@@ -25,9 +25,10 @@
 //     different lengths leaves compute units idle, and a captured call adapts while lengths grow.  A part is written as
 //     (m, l, o) in 32 bits and a second kernel joins the parts.  Short caches (and many of them) take one workgroup each.
 //
-// 100003 positions, 32 / 8 heads of 128: 82 us, 5.0 TB/s, what a copy reaches.  64 x 577 positions, 16 heads of 64: 33.8 us,
-// 4.5 TB/s.  12 x 5 tokens over ragged caches of up to 8009: 25.3 us, 2.3 TB/s; a wave has three or four tiles there, and what
-// precedes its first and follows its last one (page table, join of the waves, 5 us for the parts) is as long as their stream.
+// 100003 positions, 32 / 8 heads of 128: 83 us, 5.0 TB/s, what a copy reaches.  64 x 577 positions, 16 heads of 64: 34.0 us,
+// 4.5 TB/s.  12 x 5 tokens over ragged caches of up to 8009: 25.5 us, 2.3 TB/s; a wave has three or four tiles there, and what
+// precedes its first and follows its last one (page table, join of the waves, 5 us for the parts) is as long as their stream
+// and hidden by nothing: with three row tiles of 128 dimensions a wave has 361 registers and its SIMD to itself.
 #include "common.h"
 #include "decode_abi.h"
 
