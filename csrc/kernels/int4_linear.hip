@@ -13,9 +13,11 @@
 // where sum x comes from one more matrix instruction (its other operand is all ones), so scale and zero cost one fused
 // multiply-add per group and output, not one per weight.  All sums are fp32; at this offset the difference is as exact as a
 // sum of the weights' own products (1 to 3e-7 of a layer's typical output).  In the lowest bits codes would need one shift less
-// and stand for 128 + c and 1024 + c: 24 x 8192 x 28672 39.4 instead of 39.9 us, and 1e-6 and 2e-5 off.  An infinity in x would make that difference
-// NaN, and so would bf16 values near the end of their range, whose sums with the offset overflow: an output that is no
-// finite number is summed once more without the offset (plain4; 24 x 8192 x 28672 with an infinity in a row: 2.4 ms).
+// and stand for 128 + c and 1024 + c: 24 x 8192 x 28672 39.4 instead of 39.9 us, and 1e-6 and 2e-5 off.
+//
+// An infinity in x would make that difference NaN, and so would bf16 values near the end of their range, whose sums with the
+// offset overflow: an output that is no finite number is summed once more without the offset (plain4; 24 x 8192 x 28672 with
+// an infinity in a row: 2.4 ms).
 //
 // The waves of a workgroup share R tiles of 16 outputs and split K between them, 128 features at a time; their sums meet in
 // LDS.  The next step's loads are in flight while a step is computed.

@@ -3,7 +3,8 @@ or a few new tokens per sequence over the cache.  GPU: csrc/kernels/paged_append
 through csrc/bind/decode_ops.cpp; CPU tensors: plain PyTorch fp32 (also the oracle in tests).
 
 The cache of a layer is two tensors ``k_pages``, ``v_pages`` [pages, page, kv_heads, D] (bf16 or fp16; views of one
-buffer are fine as long as D is contiguous, strides are multiples of 8 and a page's slots lie within 2 GB, 16 MB apart at most).  Sequence ``b`` keeps position ``p`` in slot
+buffer are fine as long as D is contiguous, strides are multiples of 8 and the slots of a page lie within 2 GB, 16 MB apart
+at most).  Sequence ``b`` keeps position ``p`` in slot
 ``p % page`` of page ``table[b, p // page]``; ``table`` is int32 [B, width], so a sequence holds at most ``width * page``
 tokens.  ``lens`` (int32 [B], on the device) is the number of tokens kept BEFORE a step: both operators take the same
 ``lens`` within one step, and the caller adds to it afterwards (one token per step, or what ``ops.draft.verify_draft``
